@@ -45,7 +45,9 @@ typedef enum {
 #define SVX_STATUS_NAN_LOGITS     0x2u  /* a score or probability was NaN */
 #define SVX_STATUS_WAIT_TIMEOUT   0x4u  /* a bounded spin-wait gave up (kernel skipped its work) */
 
-typedef enum { SVX_F32 = 0, SVX_BF16 = 1 } svx_dtype;
+#define SVX_STATUS_BAD_PAGE       0x8u  /* paged cache: a page id outside the pool, or a length outside the table */
+
+typedef enum { SVX_F32 = 0, SVX_BF16 = 1, SVX_F16 = 2, SVX_I32 = 3, SVX_I64 = 4 } svx_dtype;
 
 SVX_API const char* svx_last_error(void);
 SVX_API int svx_version(void);
@@ -267,6 +269,72 @@ SVX_API int svx_attention_multi(const svx_attention_problem* problems, int count
 SVX_API int svx_attention_multi_plan_ints(int problems, int slots, int heads, int queries, int ctas);
 SVX_API int svx_attention_multi_plan(const int32_t* const* lengths, const int* keys, int problems, int slots,
                                      int heads, int queries, int ctas, int32_t* plan, int capacity);
+
+/* -------------------------------------------------------------------------------- rotary positions, paged cache */
+
+#define SVX_ROPE_INTERLEAVED 0  /* pair j = values 2j, 2j + 1 of the head (the layout of SVX_EPI_ROPE) */
+#define SVX_ROPE_HALF        1  /* pair j = values j, j + rot / 2 */
+
+/* The rotation of a head's first `rot` values: pair j of a row at position x turns by x * inv_freq[j] and is multiplied
+ * by `scale`. With several axes the pairs are split evenly among them, axis-major, and a row has one position for each
+ * (the axial rotation of `streamvoxel/models/unconditional_md4_timefree.py:24-30`: 3 axes, interleaved). */
+typedef struct {
+  const double* inv_freq;    /* device [rot / 2] */
+  int rot;                   /* even, at most the head's dim and 512 */
+  int layout;                /* SVX_ROPE_* */
+  int axes;                  /* divides rot / 2 */
+  float scale;
+  const void* positions;     /* device [tokens][axes]; NULL: the position in the cache (svx_paged_append, one axis) */
+  int position_type;         /* SVX_I32, SVX_I64 or SVX_F32 */
+} svx_rotary;
+
+/* out = rotation of x, both [tokens][heads][dim] of fp32, bf16 or fp16 with strides in elements (values of a head are
+ * contiguous); values past rot are copied. inverse != 0: the transposed rotation, which takes a gradient of out to the
+ * gradient of x. Angles are formed in float64, values computed in fp32 and rounded once. out may be x. */
+SVX_API int svx_rope(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, void* out,
+                     int64_t out_token_stride, int64_t out_head_stride, int tokens, int heads, int dim,
+                     const svx_rotary* rotary, int inverse, void* stream);
+
+/* A paged cache of keys and values: two pools [pages][kv_heads][page][dim] (bf16 or fp16, 16-byte aligned), the page ids
+ * of every sequence in order, and the new tokens' division among the sequences. Sequence s owns the new rows
+ * [offsets[s], offsets[s + 1]) and has lengths[s] keys in all, the new ones last. Rows outside of every sequence (before
+ * offsets[0], from offsets[sequences] on) are left alone in every output. The arrays are read on the device only, so a
+ * captured call follows their contents. */
+typedef struct {
+  void *k, *v;
+  int dtype;                 /* SVX_BF16 or SVX_F16 */
+  int pages, kv_heads;
+  int page;                  /* keys of a page: 16, 32, .. 1024 */
+  int dim;                   /* a multiple of 8 */
+  int sequences, table_width;
+  const int32_t* table;      /* device [sequences][table_width] page ids */
+  const int32_t* lengths;    /* device [sequences] */
+  const int32_t* offsets;    /* device [sequences + 1], ascending */
+  uint32_t* status;          /* optional device [sequences]: SVX_STATUS_BAD_PAGE is OR-ed in */
+} svx_paged_cache;
+
+/* Stores new keys and values, each [tokens][kv_heads][dim] of the cache's type: row i of sequence s goes to key
+ * lengths[s] - (offsets[s + 1] - offsets[s]) + i. rotary (optional) turns the keys on the way and, where given, q
+ * [tokens][q_heads][dim] into q_out (contiguous), in the same launch. A key whose place is outside the table, or whose
+ * page id is outside the pool, is not stored and sets SVX_STATUS_BAD_PAGE. */
+SVX_API int svx_paged_append(const svx_paged_cache* cache, const void* k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                             int tokens, const svx_rotary* rotary, const void* q, int64_t q_token_stride,
+                             int64_t q_head_stride, int q_heads, void* q_out, void* stream);
+
+/* Attention of the new tokens over their sequences' keys, dim 64, 96 or 128: out [tokens][q_heads][dim] =
+ * softmax(scale q k^T) v, kv head = q head / (q_heads / kv_heads). causal != 0: row i of a sequence with n new rows sees
+ * the keys up to lengths - n + i; else all. A row that sees no key gives 0. lse (optional) [tokens][q_heads]: the natural
+ * logarithm of the row's sum of exponentials, -inf for such a row. What the pages hold past a sequence's length is not
+ * read. Lengths outside the table are clamped to it and page ids outside the pool count as keys and values of 0; both
+ * set SVX_STATUS_BAD_PAGE. max_query: the most new rows of a sequence that the caller expects (0: unknown); it picks the
+ * form of the kernel and never changes what is computed. workspace: svx_paged_attention_workspace_bytes of device
+ * scratch for the same arguments, for this call alone while it runs; nothing is kept in it between calls. */
+SVX_API size_t svx_paged_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int dim,
+                                                   int max_query);
+SVX_API int svx_paged_attention(const svx_paged_cache* cache, const void* q, int64_t q_token_stride,
+                                int64_t q_head_stride, int tokens, int q_heads, int causal, float scale, void* out,
+                                float* lse, int max_query, void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ the engine */
 

@@ -15,8 +15,9 @@ LIBRARY = os.path.join(PACKAGE, 'libsvx.so')
 HEADER = os.path.join(os.path.dirname(PACKAGE), 'include', 'svx.h')
 
 SVX_OK, SVX_ERR_INVALID, SVX_ERR_CUDA, SVX_ERR_UNSUPPORTED = 0, 1, 2, 3
-STATUS_QUOTA_MISSED, STATUS_NAN_LOGITS, STATUS_WAIT_TIMEOUT = 0x1, 0x2, 0x4
-F32, BF16 = 0, 1
+STATUS_QUOTA_MISSED, STATUS_NAN_LOGITS, STATUS_WAIT_TIMEOUT, STATUS_BAD_PAGE = 0x1, 0x2, 0x4, 0x8
+F32, BF16, F16, I32, I64 = range(5)
+ROPE_LAYOUTS = dict(interleaved=0, half=1)
 EPI_BIAS, EPI_BIAS_GELU, EPI_GATE_RESIDUAL, EPI_RESIDUAL, EPI_ROPE, EPI_CLASS_MAJOR = range(6)
 
 c_ptr = ctypes.c_void_p
@@ -75,6 +76,19 @@ class AttentionProblem(ctypes.Structure):
                 ('out', c_ptr)]
 
 
+class Rotary(ctypes.Structure):
+    """`svx_rotary`."""
+    _fields_ = [('inv_freq', c_ptr), ('rot', c_int), ('layout', c_int), ('axes', c_int), ('scale', ctypes.c_float),
+                ('positions', c_ptr), ('position_type', c_int)]
+
+
+class PagedCache(ctypes.Structure):
+    """`svx_paged_cache`."""
+    _fields_ = [('k', c_ptr), ('v', c_ptr)] + \
+               [(n, c_int) for n in ('dtype', 'pages', 'kv_heads', 'page', 'dim', 'sequences', 'table_width')] + \
+               [(n, c_ptr) for n in ('table', 'lengths', 'offsets', 'status')]
+
+
 class EngineWorkspace(ctypes.Structure):
     _fields_ = [(n, c_ptr) for n in ('xb', 'xc', 'h', 'qkv', 'attn', 'mlp', 'qx', 'ax', 'stats_b', 'stats_c')]
 
@@ -114,6 +128,13 @@ _SIGNATURES = {
     'svx_attention_multi_plan_ints': (c_int, [c_int, c_int, c_int, c_int, c_int]),
     'svx_attention_multi_plan': (c_int, [ctypes.POINTER(c_ptr), ctypes.POINTER(c_int), c_int, c_int, c_int, c_int,
                                          c_int, c_ptr, c_int]),
+    'svx_rope': (c_int, [c_ptr, c_int, c_i64, c_i64, c_ptr, c_i64, c_i64, c_int, c_int, c_int, ctypes.POINTER(Rotary),
+                         c_int, c_ptr]),
+    'svx_paged_append': (c_int, [ctypes.POINTER(PagedCache), c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_int,
+                                 ctypes.POINTER(Rotary), c_ptr, c_i64, c_i64, c_int, c_ptr, c_ptr]),
+    'svx_paged_attention_workspace_bytes': (ctypes.c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    'svx_paged_attention': (c_int, [ctypes.POINTER(PagedCache), c_ptr, c_i64, c_i64, c_int, c_int, c_int,
+                                    ctypes.c_float, c_ptr, c_ptr, c_int, c_ptr, c_ptr]),
     'svx_engine_create': (c_int, [ctypes.POINTER(EngineConfig), ctypes.POINTER(EngineWeights),
                                   ctypes.POINTER(EngineWorkspace), ctypes.POINTER(c_ptr)]),
     'svx_engine_forward': (c_int, [c_ptr, c_int, c_ptr, c_ptr, c_ptr]),

@@ -1,0 +1,569 @@
+// Attention of new tokens over a paged cache: the form for few query rows (decoding), the joining kernel, and the
+// entry point that picks the form.
+//
+//   out[row] = softmax(scale q k^T) v over the keys that the row sees, kv head = head / group
+//
+// One pass over the keys with a running maximum m and sum l per row; o, m and l stay in fp32 registers:
+//   m' = max(m, max s), o = o 2^(m - m') + p v, l = l 2^(m - m') + sum p, p = 2^(s - m')
+// (s in log2 units). The weights p are rounded to the cache's type for the product with v, while l sums them
+// unrounded: the rounding of each weight (2^-9 bf16, 2^-12 fp16) is random and averages out over keys, and a row with
+// one dominant key has p = 1 there, which is exact. For fp16, whose least step is 2^-24, weights are held 2^7 larger.
+//
+// Bound: the keys and values are read once for the whole group of query heads that share them, so a step with few rows
+// is bound by memory. A group's rows are packed into one 16-row matrix tile (mma.sync m16n8k16; the tensor work is a
+// small fraction of its rate, and tcgen05's 128-row tiles would be 7/8 padding). The line of all 64-key tiles of the
+// batch (paged.cuh) is cut into equal runs, one per CTA, two CTAs a SM: unequal lengths, one long sequence or many
+// short ones all load the card evenly. Each of a CTA's four warps streams its own 16 keys of every tile through a
+// private ring of cp.async stages, so the loop has no block barrier; the warps' parts of a unit are merged through
+// shared memory at its end.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace svx {
+
+int check_cache(const svx_paged_cache* c, const char* who, int* shift) {
+  const std::string at = std::string(who) + ": ";
+  SVX_REQUIRE(c, at + "null cache");
+  SVX_REQUIRE(c->dtype == SVX_BF16 || c->dtype == SVX_F16, at + "the cache must be bf16 or fp16");
+  SVX_REQUIRE(c->pages > 0 && c->kv_heads > 0 && c->kv_heads <= 1024, at + "bad page or head count");
+  SVX_REQUIRE(c->dim > 0 && c->dim % 8 == 0 && c->dim <= 1024, at + "dim must be a multiple of 8, at most 1024");
+  SVX_REQUIRE(c->page >= 16 && c->page <= 1024 && (c->page & (c->page - 1)) == 0,
+              at + "a page must hold 16, 32, .. 1024 keys");
+  SVX_REQUIRE(c->sequences >= 0 && c->sequences <= (1 << 20), at + "bad sequence count");
+  SVX_REQUIRE(c->table_width > 0 && (int64_t)c->table_width * c->page <= (1 << 30), at + "bad table width");
+  SVX_REQUIRE(c->k && c->v && (!c->sequences || (c->table && c->lengths && c->offsets)), at + "null cache arrays");
+  SVX_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) == 0,
+              at + "pools must be 16-byte aligned");
+  *shift = 0;
+  while ((1 << *shift) < c->page) ++*shift;
+  return SVX_OK;
+}
+
+namespace paged {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 16;
+constexpr int kCtasPerSm = 2;
+
+template <typename T> struct Half;   // the two 16-bit types
+template <> struct Half<__nv_bfloat16> {
+  static constexpr float shift = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+    return d;
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Half<__half> {
+  static constexpr float shift = 7.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+    return d;
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes to shared memory, zeros where !take (the source is then not read).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0)
+               : "memory");
+}
+
+template <int D> struct Shape {
+  static constexpr int chunks = D / 8;                  // 16-byte pieces of a row
+  static constexpr int row_bytes = (chunks + 1) * 16;   // odd in 16-byte units: ldmatrix rows fall into distinct banks
+  static constexpr int stage_bytes = 2 * 16 * row_bytes;
+  // Enough keys in flight for the memory's latency (about 64 KB a SM) with two CTAs a SM: measured below.
+  static constexpr int stages = D == 64 ? 6 : D == 96 ? 4 : 3;
+  static constexpr int merge_stride = 40;               // floats of a merged row's 32 values, padded
+  static constexpr size_t smem =
+      (size_t)kWarps * stages * stage_bytes + (size_t)kWarps * kRows * merge_stride * 4;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Params p) {
+  using S = Shape<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ PlanShared plan_shared;
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  float* merge = reinterpret_cast<float*>(smem + kWarps * S::stages * S::stage_bytes);
+  const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
+  const uint32_t ring = smem_addr(smem + warp * S::stages * S::stage_bytes);
+  grid_launch_dependents();
+  grid_dependency_wait();
+  plan<kThreads>(p, cta, gridDim.x, plan_shared);
+  const Place& place = plan_shared.place;
+  const int count = (int)(place.end - place.begin);
+  if (threadIdx.x == 0) {
+    Join* join = reinterpret_cast<Join*>(p.join) + cta;
+    join->valid = 0;
+  }
+  if (count <= 0) return;
+
+  // The loading side: a cursor up to stages - 1 tiles ahead, with the next slice's page id already on its way.
+  Cursor ahead;
+  ahead.set(p, place.s, place.j, place.h);
+  int ahead_t = place.t, issued = 0, page = 0;
+  auto look_up = [&] {
+    const int key = ahead_t * kTile + warp * 16;
+    page = key < ahead.limit ? __ldg(p.table + (int64_t)ahead.s * p.table_width + (key >> p.page_shift)) : 0;
+  };
+  look_up();
+  auto issue = [&] {
+    if (issued < count) {
+      const int key = ahead_t * kTile + warp * 16;
+      int valid = max(0, min(16, ahead.limit - key));
+      if (page < 0 || page >= p.pages) {
+        if (p.status && lane == 0) atomicOr(p.status + ahead.s, SVX_STATUS_BAD_PAGE);
+        page = 0;
+        valid = 0;
+      }
+      const int head = ahead.h / p.blocks;
+      const int64_t row = (((int64_t)page * p.kv_heads + head) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+      const T* k = static_cast<const T*>(p.k) + row * D;
+      const T* v = static_cast<const T*>(p.v) + row * D;
+      const uint32_t stage = ring + issued % S::stages * S::stage_bytes;
+#pragma unroll
+      for (int i = 0; i < S::chunks / 2; ++i) {
+        const int e = lane + 32 * i, r = e / S::chunks, c = e % S::chunks;
+        copy16(stage + r * S::row_bytes + c * 16, k + r * D + c * 8, r < valid);
+      }
+#pragma unroll
+      for (int i = 0; i < S::chunks / 2; ++i) {
+        const int e = lane + 32 * i, r = e / S::chunks, c = e % S::chunks;
+        copy16(stage + 16 * S::row_bytes + r * S::row_bytes + c * 16, v + r * D + c * 8, r < valid);
+      }
+      ++issued;
+      if (++ahead_t == ahead.tiles) {
+        ahead_t = 0;
+        ahead.next(p);
+      }
+      if (issued < count) look_up();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < S::stages - 1; ++i) issue();
+
+  Cursor at;
+  at.set(p, place.s, place.j, place.h);
+  int t = place.t, segment = 0;
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4], m[2], l[2];
+  int limit[2];
+  bool fresh = true;
+  for (int i = 0; i < count; ++i) {
+    if (fresh) {
+      fresh = false;
+      if (threadIdx.x == 0 && p.status) {
+        const int raw = __ldg(p.lengths + at.s);
+        if (raw != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
+      }
+      const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
+      const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = lane / 4 + 8 * u, token = r / part;
+        const bool live = token < tokens;
+        limit[u] = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token0 + token + 1)) : at.q.len;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)(at.q.row0 + token0 + token) * p.q_token +
+                     (int64_t)(at.h / p.blocks * p.group + g0 + r - token * part) * p.q_head + lane % 4 * 2;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[kk][u] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16)) : 0u;
+          qf[kk][u + 2] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16 + 8)) : 0u;
+        }
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::stages - 2) : "memory");
+    __syncwarp();
+    issue();   // into the stage read last time round
+    const uint32_t stage = ring + i % S::stages * S::stage_bytes;
+
+    // S = Q K^T: K's rows are the columns of the product. Lanes 0-15 address keys 0-7, 16-31 keys 8-15; every other
+    // eight the second half of 16 dims.
+    float s[2][4] = {};
+    const uint32_t k_at = stage + ((lane & 7) + (lane >> 4) * 8) * S::row_bytes + ((lane >> 3) & 1) * 16;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t b[4];
+      ldmatrix4(b, k_at + kk * 32);
+      Half<T>::mma(s[0], qf[kk], b[0], b[1]);
+      Half<T>::mma(s[1], qf[kk], b[2], b[3]);
+    }
+    const int key0 = t * kTile + warp * 16 + lane % 4 * 2;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float& x = s[nt][e];
+        x = key0 + nt * 8 + (e & 1) < limit[e >> 1] ? x * p.scale_log2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], x);
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+    }
+    const bool grows = top[0] > m[0] || top[1] > m[1];
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float now = fmaxf(m[u], top[u]);
+        const float f = m[u] == now ? 1.f : exp2_approx(m[u] - now);   // m = -inf: 0
+        m[u] = now;
+        l[u] *= f;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          o[d][2 * u] *= f;
+          o[d][2 * u + 1] *= f;
+        }
+      }
+    }
+    float w[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float base = m[u] == -INFINITY ? 0.f : m[u] - Half<T>::shift;   // a row without keys so far: weights 0
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = exp2_approx(s[nt][2 * u + e] - base);
+          w[nt][2 * u + e] = x;
+          l[u] += x;
+        }
+    }
+    const uint32_t a[4] = {Half<T>::pack(w[0][0], w[0][1]), Half<T>::pack(w[0][2], w[0][3]),
+                           Half<T>::pack(w[1][0], w[1][1]), Half<T>::pack(w[1][2], w[1][3])};
+    const uint32_t v_at = stage + 16 * S::row_bytes + (lane & 15) * S::row_bytes + (lane >> 4) * 16;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      uint32_t b[4];
+      ldmatrix4_trans(b, v_at + d * 32);
+      Half<T>::mma(o[2 * d], a, b[0], b[1]);
+      Half<T>::mma(o[2 * d + 1], a, b[2], b[3]);
+    }
+    ++t;
+    if (t < at.tiles && i + 1 < count) continue;
+
+    // The unit's end, or the run's: merge the warps' parts.
+    const bool whole = (segment || place.t == 0) && t == at.tiles;
+    const int slot = 2 * cta + (segment ? 1 : 0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      if (lane % 4 == 0) {
+        s_m[warp][lane / 4 + 8 * u] = m[u];
+        s_l[warp][lane / 4 + 8 * u] = l[u];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = lane / 4 + 8 * u;
+      float now = s_m[0][r];
+#pragma unroll
+      for (int x = 1; x < kWarps; ++x) now = fmaxf(now, s_m[x][r]);
+      const float f = m[u] == now ? 1.f : exp2_approx(m[u] - now);
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) {
+        o[d][2 * u] *= f;
+        o[d][2 * u + 1] *= f;
+      }
+    }
+    // One row and four of its columns a thread, 32 columns a round.
+    const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
+    float top_r = s_m[0][r], sum_r = 0.f;
+#pragma unroll
+    for (int x = 1; x < kWarps; ++x) top_r = fmaxf(top_r, s_m[x][r]);
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x)
+      sum_r += s_m[x][r] == top_r ? s_l[x][r] : s_l[x][r] * exp2_approx(s_m[x][r] - top_r);
+    const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
+    const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+    const bool live = r < tokens * part;
+    const int64_t out_row = (int64_t)(at.q.row0 + token0 + r / part) * p.q_heads + at.h / p.blocks * p.group + g0 + r % part;
+    const float inverse = sum_r == 0.f ? 0.f : 1.f / sum_r;
+#pragma unroll
+    for (int round = 0; round < D / 32; ++round) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<float2*>(merge + (warp * kRows + lane / 4 + 8 * u) * S::merge_stride + d * 8 + lane % 4 * 2) =
+              make_float2(o[round * 4 + d][2 * u], o[round * 4 + d][2 * u + 1]);
+      __syncthreads();
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float4 f = *reinterpret_cast<const float4*>(merge + (x * kRows + r) * S::merge_stride + c);
+        sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(p.partial_o + ((int64_t)slot * p.rows + r) * D + round * 32 + c) = sum;
+      } else if (live) {
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + round * 32 + c) =
+            make_uint2(Half<T>::pack(sum.x * inverse, sum.y * inverse), Half<T>::pack(sum.z * inverse, sum.w * inverse));
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x % 8 == 0) {
+      if (!whole) {
+        p.partial_ml[(int64_t)slot * p.rows + r] = make_float2(top_r, sum_r);
+      } else if (live && p.lse) {
+        p.lse[out_row] = sum_r == 0.f ? -INFINITY : (top_r - Half<T>::shift + log2f(sum_r)) * 0.69314718056f;
+      }
+    }
+    if (threadIdx.x == 0 && segment == 0 && !whole && t == at.tiles) {
+      Join* join = reinterpret_cast<Join*>(p.join) + cta;
+      const int64_t first = place.unit / place.each;
+      join->s = at.s;
+      join->j = at.j;
+      join->h = at.h;
+      join->first = (int)first;
+      join->first_slot = place.unit == first * place.each ? 0 : 1;
+      join->valid = 1;
+    }
+    ++segment;
+    t = 0;
+    at.next(p);
+    fresh = true;
+  }
+}
+
+// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, rows
+// 4 y to 4 y + 3, two warps a row that share its parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+  grid_dependency_wait();
+  const Join join = reinterpret_cast<const Join*>(p.join)[blockIdx.x];
+  if (!join.valid) return;
+  __shared__ float4 s_o[8][32];
+  __shared__ float2 s_ml[8];
+  Cursor at;
+  at.set(p, join.s, join.j, join.h);
+  const int warp = warp_id(), lane = lane_id(), r = blockIdx.y * 4 + warp / 2, c = blockIdx.x;
+  const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
+  const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+  const bool live = r < tokens * part;
+  const int parts = c - join.first + 1;
+  auto slot = [&](int i) { return 2 * (join.first + i) + (i == 0 ? join.first_slot : 0); };
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, total = 0.f;
+  if (live) {
+    for (int i0 = warp & 1; i0 < parts; i0 += 64) {
+      const int i = i0 + 2 * lane;   // this warp's parts: every second one
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (i < parts) ml = p.partial_ml[(int64_t)slot(i) * p.rows + r];
+      float now = ml.x;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+      now = fmaxf(now, top);
+      const float old = top == now ? 1.f : exp2_approx(top - now);
+      const float f = ml.x == now ? 1.f : exp2_approx(ml.x - now);
+      float add = ml.y * f;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+      total = total * old + add;
+      sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+      top = now;
+      const int here = min(32, (parts - i0 + 1) / 2);
+#pragma unroll 8
+      for (int x = 0; x < here; ++x) {
+        const float fx = __shfl_sync(0xffffffffu, f, x);
+        if (lane < D / 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.partial_o + ((int64_t)slot(i0 + 2 * x) * p.rows + r) * D + 4 * lane);
+          sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
+          sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
+        }
+      }
+    }
+  }
+  s_o[warp][lane] = sum;
+  if (lane == 0) s_ml[warp] = make_float2(top, total);
+  __syncthreads();
+  if (!live || (warp & 1)) return;
+  const float2 other = s_ml[warp + 1];
+  const float4 v = s_o[warp + 1][lane];
+  const float now = fmaxf(top, other.x);
+  const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
+  total = total * f + other.y * g;
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  const int64_t out_row = (int64_t)(at.q.row0 + token0 + r / part) * p.q_heads + at.h / p.blocks * p.group + g0 + r % part;
+  if (lane < D / 4)
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
+        make_uint2(Half<T>::pack((sum.x * f + v.x * g) * inverse, (sum.y * f + v.y * g) * inverse),
+                   Half<T>::pack((sum.z * f + v.z * g) * inverse, (sum.w * f + v.w * g) * inverse));
+  if (lane == 0 && p.lse)
+    p.lse[out_row] = total == 0.f ? -INFINITY : (now - Half<T>::shift + log2f(total)) * 0.69314718056f;
+}
+
+int sm_count(int* sms) {
+  static PerDevice<int> per_device;
+  return per_device.get(sms, [](int device, int* count) -> int {
+    SVX_CHECK_CUDA(cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device));
+    return SVX_OK;
+  });
+}
+
+template <typename T, int D>
+int few_rows_launch(const Params& p, int ctas, cudaStream_t stream) {
+  static PerDevice<int> ready;
+  int unused;
+  const int rc = ready.get(&unused, [](int, int*) -> int {
+    SVX_CHECK_CUDA(cudaFuncSetAttribute(few_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D>::smem));
+    return SVX_OK;
+  });
+  if (rc) return rc;
+  return launch_dependent("few_rows_kernel", few_rows_kernel<T, D>, dim3(ctas), dim3(kThreads), Shape<D>::smem, stream, p);
+}
+
+template <typename T>
+int launch_all(const Params& p, int dim, int ctas, cudaStream_t stream) {
+  const dim3 grid(ctas, (p.rows + 3) / 4);
+  int rc;
+  if (dim == 64) rc = few_rows_launch<T, 64>(p, ctas, stream);
+  else if (dim == 96) rc = few_rows_launch<T, 96>(p, ctas, stream);
+  else rc = few_rows_launch<T, 128>(p, ctas, stream);
+  if (rc) return rc;
+  if (dim == 64) return launch_dependent("join_kernel", join_kernel<T, 64>, grid, dim3(256), 0, stream, p);
+  if (dim == 96) return launch_dependent("join_kernel", join_kernel<T, 96>, grid, dim3(256), 0, stream, p);
+  return launch_dependent("join_kernel", join_kernel<T, 128>, grid, dim3(256), 0, stream, p);
+}
+
+// How a call is divided: set from its shape alone, so that the workspace's size and the launch agree.
+struct Division {
+  int group_part, blocks, unit_tokens, rows, ctas, min_tiles;
+};
+
+int divide(int group, Division* d) {
+  int sms = 0;
+  if (const int rc = sm_count(&sms)) return rc;
+  d->group_part = std::min(group, kRows);
+  d->blocks = (group + kRows - 1) / kRows;
+  d->unit_tokens = kRows / d->group_part;
+  d->rows = kRows;
+  d->ctas = sms * kCtasPerSm;
+  d->min_tiles = 2;
+  return SVX_OK;
+}
+
+size_t workspace_bytes(const Division& d, int dim) {
+  return (size_t)d.ctas * (sizeof(Join) + 2 * (size_t)d.rows * (dim * sizeof(float) + sizeof(float2)));
+}
+
+int check_attention(int tokens, int q_heads, int kv_heads, int dim) {
+  SVX_REQUIRE(dim == 64 || dim == 96 || dim == 128, "svx_paged_attention: dim must be 64, 96 or 128");
+  SVX_REQUIRE(kv_heads > 0 && q_heads > 0 && q_heads % kv_heads == 0 && q_heads <= 4096,
+              "svx_paged_attention: the query heads must be a multiple of the cache's");
+  SVX_REQUIRE(tokens >= 0, "svx_paged_attention: bad token count");
+  return SVX_OK;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace svx
+
+using namespace svx;
+
+extern "C" size_t svx_paged_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int dim,
+                                                      int max_query) {
+  (void)sequences; (void)max_query;
+  if (paged::check_attention(tokens, q_heads, kv_heads, dim)) return 0;
+  paged::Division d;
+  if (paged::divide(q_heads / kv_heads, &d)) return 0;
+  return paged::workspace_bytes(d, dim);
+}
+
+extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, int64_t q_token_stride,
+                                   int64_t q_head_stride, int tokens, int q_heads, int causal, float scale, void* out,
+                                   float* lse, int max_query, void* workspace, void* stream) {
+  int shift = 0;
+  if (const int rc = check_cache(cache, "svx_paged_attention", &shift)) return rc;
+  if (const int rc = paged::check_attention(tokens, q_heads, cache->kv_heads, cache->dim)) return rc;
+  SVX_REQUIRE(scale > 0.f && scale <= 1e30f, "svx_paged_attention: scale must be positive and finite");
+  (void)max_query;
+  if (!tokens || !cache->sequences) return SVX_OK;
+  SVX_REQUIRE(q && out && workspace, "svx_paged_attention: null arguments");
+  SVX_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
+              "svx_paged_attention: strides of q must be multiples of 8 elements");
+  SVX_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u) == 0,
+              "svx_paged_attention: operands must be 16-byte aligned");
+  paged::Division d;
+  if (const int rc = paged::divide(q_heads / cache->kv_heads, &d)) return rc;
+  paged::Params p{};
+  p.q = q;
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.k = cache->k;
+  p.v = cache->v;
+  p.table = cache->table;
+  p.lengths = cache->lengths;
+  p.offsets = cache->offsets;
+  p.out = out;
+  p.lse = lse;
+  p.status = cache->status;
+  const size_t slots = 2 * (size_t)d.ctas * d.rows;
+  p.partial_o = static_cast<float*>(workspace);
+  p.partial_ml = reinterpret_cast<float2*>(p.partial_o + slots * cache->dim);
+  p.join = reinterpret_cast<int32_t*>(p.partial_ml + slots);
+  p.tokens = tokens;
+  p.sequences = cache->sequences;
+  p.q_heads = q_heads;
+  p.kv_heads = cache->kv_heads;
+  p.group = q_heads / cache->kv_heads;
+  p.page_shift = shift;
+  p.pages = cache->pages;
+  p.table_width = cache->table_width;
+  p.causal = causal != 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.unit_tokens = d.unit_tokens;
+  p.blocks = d.blocks;
+  p.group_part = d.group_part;
+  p.rows = d.rows;
+  p.min_tiles = d.min_tiles;
+  if (cache->dtype == SVX_BF16) return paged::launch_all<__nv_bfloat16>(p, cache->dim, d.ctas, as_stream(stream));
+  return paged::launch_all<__half>(p, cache->dim, d.ctas, as_stream(stream));
+}

@@ -5,6 +5,7 @@ Each wrapper validates dtypes/shapes on the host and calls exactly one C-ABI fun
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -311,4 +312,227 @@ def attention(q, k, v, slots, heads, queries, keys, *, q_row_stride, kv_slot_str
                                     kv_row_stride, ptr(lengths), slots, heads, queries, keys, ptr(out), ptr(table),
                                     ctas, stream_ptr()),
           'svx_attention')
+    return out
+
+
+# ------------------------------------------------------------------------- rotary positions and the paged cache
+
+_ROW_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_POSITION_DTYPES = {torch.int32: _lib.I32, torch.int64: _lib.I64, torch.float32: _lib.F32}
+
+
+def _need(ok, text):
+    if not ok:
+        raise ValueError(text)
+
+
+def _device_of(*tensors):
+    """The one CUDA device of the tensors (None entries apart)."""
+    devices = {t.device for t in tensors if t is not None}
+    _need(len(devices) == 1 and next(iter(devices)).type == 'cuda', 'operands must be on one CUDA device')
+    return devices.pop()
+
+
+def _rows(name, t, tokens=None, heads=None, dim=None, dtype=None):
+    """A [tokens, heads, dim] operand with contiguous rows; the token and head strides are free."""
+    _need(t.ndim == 3, f'{name} must be [tokens, heads, dim]')
+    for size, want, what in zip(t.shape, (tokens, heads, dim), ('tokens', 'heads', 'dim')):
+        _need(want is None or size == want, f'{name} has {size} {what}, expected {want}')
+    _need(dtype is None or t.dtype == dtype, f'{name} must be {dtype}')
+    _need(t.stride(2) == 1 or t.shape[2] == 1, f'{name} must have contiguous rows (stride 1 in dim)')
+
+
+def _rotary(inv_freq, positions, tokens, dim, layout, scale):
+    _need(inv_freq.dtype == torch.float64 and inv_freq.ndim == 1 and inv_freq.is_contiguous(),
+          'inv_freq must be a contiguous float64 vector, one entry per pair')
+    pairs = inv_freq.numel()
+    _need(0 < 2 * pairs <= dim, f'{pairs} pairs do not fit heads of {dim}')
+    _need(layout in _lib.ROPE_LAYOUTS, f'layout must be one of {sorted(_lib.ROPE_LAYOUTS)}')
+    axes, kind = 1, _lib.I64
+    if positions is not None:
+        _need(positions.dtype in _POSITION_DTYPES, 'positions must be int32, int64 or float32')
+        _need(positions.ndim in (1, 2) and positions.shape[0] == tokens and positions.is_contiguous(),
+              f'positions must be a contiguous [{tokens}] or [{tokens}, axes] tensor')
+        axes = positions.shape[1] if positions.ndim == 2 else 1
+        kind = _POSITION_DTYPES[positions.dtype]
+        _need(axes > 0 and pairs % axes == 0, f'{axes} axes do not share {pairs} pairs evenly')
+    _need(math.isfinite(scale), 'the rotary scale must be finite')
+    return _lib.Rotary(inv_freq.data_ptr(), 2 * pairs, _lib.ROPE_LAYOUTS[layout], axes, float(scale),
+                       ptr(positions), kind)
+
+
+def rope_frequencies(rot, base=10000.0, *, axes=1, scaling=None, factor=1.0, original=8192, device='cuda'):
+    """(inv_freq [rot / 2] float64, scale) of `rope` and `paged_append`: base^(-2j / width) with width = rot / axes,
+    repeated for every axis. `scaling` stretches the positions a model was trained on (`original` of them) by `factor`:
+    'linear' divides every frequency by it; 'base' enlarges the base so that the slowest pair is divided by it and the
+    fastest keeps its angle; 'by_parts' keeps the pairs that turn at least 32 times within `original` positions, divides
+    those that turn at most once, blends between, and gives scale = 0.1 ln(factor) + 1. Otherwise scale is 1."""
+    _need(rot > 0 and axes > 0 and rot % (2 * axes) == 0, f'rot ({rot}) must be a positive multiple of 2 x {axes} axes')
+    _need(scaling in (None, 'linear', 'base', 'by_parts'), f'unknown scaling {scaling!r}')
+    _need(base > 0 and factor >= 1 and original > 0, 'base and original must be positive, factor at least 1')
+    width, scale = rot // axes, 1.0
+    if scaling == 'base':
+        _need(width > 2, "scaling 'base' needs more than one pair an axis")
+        base = base * factor ** (width / (width - 2))
+    freq = float(base) ** (-np.arange(0, width, 2, dtype=np.float64) / width)
+    if scaling == 'linear':
+        freq = freq / factor
+    elif scaling == 'by_parts':
+        keep = np.clip((original * freq / (2 * math.pi) - 1) / 31, 0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+        scale = 0.1 * math.log(factor) + 1
+    return torch.from_numpy(np.tile(freq, axes)).to(device), scale
+
+
+class _Rope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, layout, scale, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.args = layout, scale, inverse
+        return rope(x, positions, inv_freq, layout=layout, scale=scale, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        layout, scale, inverse = ctx.args
+        grad = grad if grad.stride(-1) == 1 else grad.contiguous()
+        return rope(grad, *ctx.saved_tensors, layout=layout, scale=scale, inverse=not inverse), *[None] * 5
+
+
+def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=False, out=None):
+    """Rotary positions: the first 2 * len(inv_freq) values of each head of x [tokens, heads, dim] (fp32, bf16, fp16;
+    token and head strides free) turned by positions * inv_freq and multiplied by scale, the others copied.
+
+    positions: [tokens], or [tokens, axes] with the pairs split evenly among the axes (int32, int64 or float32). inv_freq:
+    float64, from `rope_frequencies`. Pairs are (2j, 2j + 1) ('interleaved') or (j, j + rot / 2) ('half'). inverse: the
+    transposed rotation, the gradient's way back; x that requires grad takes it by itself. out: a [tokens, heads, dim]
+    tensor of x's type, x itself or one that does not overlap it."""
+    _rows('x', x)
+    _need(x.dtype in _ROW_DTYPES, f'x must be fp32, bf16 or fp16, got {x.dtype}')
+    tokens, heads, dim = x.shape
+    _need(heads > 0 and dim > 0, 'x has no heads or values')
+    _need(positions is not None, 'rope needs positions')
+    rotary = _rotary(inv_freq, positions, tokens, dim, layout, scale)
+    if torch.is_grad_enabled() and x.requires_grad:
+        _need(out is None, 'out is not available for x that requires grad')
+        return _Rope.apply(x, positions, inv_freq, layout, scale, inverse)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), device=x.device, dtype=x.dtype)
+    else:
+        _rows('out', out, tokens, heads, dim, x.dtype)
+        _need(all(n == 1 or s != 0 for n, s in zip(out.shape, out.stride())), 'out must not repeat memory')
+    with torch.cuda.device(_device_of(x, positions, inv_freq, out)):
+        check(_lib.load().svx_rope(_lib.raw_ptr(x), _ROW_DTYPES[x.dtype], x.stride(0), x.stride(1), _lib.raw_ptr(out),
+                                   out.stride(0), out.stride(1), tokens, heads, dim, ctypes.byref(rotary), int(inverse),
+                                   stream_ptr()), 'svx_rope')
+    return out
+
+
+def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
+    _need(k_pages.ndim == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
+          'k_pages and v_pages must be [pages, kv_heads, page, dim] pools of one shape and type')
+    _need(k_pages.dtype in (torch.bfloat16, torch.float16), f'the cache must be bf16 or fp16, got {k_pages.dtype}')
+    pages, heads, page, dim = k_pages.shape
+    _need(page in (16, 32, 64, 128, 256, 512, 1024), f'a page must hold 16, 32, .. 1024 keys, got {page}')
+    for name, t in (('table', table), ('lengths', lengths), ('offsets', offsets), ('status', status)):
+        _need(t is None or t.dtype == torch.int32, f'{name} must be int32')
+    _need(table.ndim == 2 and table.shape[1] > 0, 'table must be [sequences, pages of a sequence]')
+    sequences = table.shape[0]
+    _need(tuple(lengths.shape) == (sequences,), f'lengths must be [{sequences}]')
+    _need(tuple(offsets.shape) == (sequences + 1,), f'offsets must be [{sequences + 1}]')
+    _need(status is None or tuple(status.shape) == (sequences,), f'status must be [{sequences}]')
+    return _lib.PagedCache(ptr(k_pages), ptr(v_pages), _ROW_DTYPES[k_pages.dtype], pages, heads, page, dim, sequences,
+                           table.shape[1], ptr(table), ptr(lengths), ptr(offsets), ptr(status))
+
+
+def _no_grad(*tensors):
+    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
+          'the paged cache takes no part in autograd: call under torch.no_grad()')
+
+
+def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=None, positions=None,
+                 layout='interleaved', rope_scale=1.0, q=None, q_out=None, status=None):
+    """Store new keys and values [tokens, kv_heads, dim] in a paged cache, the keys rotated on the way.
+
+    k_pages, v_pages: pools [pages, kv_heads, page, dim] (bf16 or fp16; a page holds 16, 32, .. 1024 keys), written in
+    place. table [sequences, n] int32: page ids in order. Sequence s owns the new rows offsets[s] .. offsets[s + 1] - 1 and
+    has lengths[s] keys with them (int32, read on the device only). Rows outside of every sequence are left alone.
+    inv_freq, layout, rope_scale and positions as in `rope`; without positions a key's place in the cache is its
+    position. q [tokens, q_heads, dim] (optional) is rotated in the same launch and returned (into q_out where given:
+    contiguous). A key whose place lies outside the table, or whose page id lies outside the pool, is not stored; status
+    [sequences] int32 (optional) gets STATUS_BAD_PAGE for its sequence. Two tokens given the same place race."""
+    cache = _paged_cache(k_pages, v_pages, table, lengths, offsets, status)
+    _rows('k', k, None, cache.kv_heads, cache.dim, k_pages.dtype)
+    _rows('v', v, k.shape[0], cache.kv_heads, cache.dim, k_pages.dtype)
+    tokens = k.shape[0]
+    _need(inv_freq is not None or (q is None and positions is None), 'q and positions need inv_freq')
+    _need(q is not None or q_out is None, 'q_out needs q')
+    rotary = None if inv_freq is None else _rotary(inv_freq, positions, tokens, cache.dim, layout, rope_scale)
+    if q is not None:
+        _rows('q', q, tokens, None, cache.dim, k_pages.dtype)
+        _need(0 < q.shape[1] <= 4096, 'q must have 1 to 4096 heads')
+        if q_out is None:
+            q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        else:
+            _rows('q_out', q_out, tokens, q.shape[1], cache.dim, q.dtype)
+    _no_grad(k, v, k_pages, v_pages, q)
+    strides = (0, 0, 0) if q is None else (q.stride(0), q.stride(1), q.shape[1])
+    with torch.cuda.device(_device_of(k, v, k_pages, v_pages, table, lengths, offsets, inv_freq, positions, q, q_out,
+                                      status)):
+        check(_lib.load().svx_paged_append(ctypes.byref(cache), _lib.raw_ptr(k), k.stride(0), k.stride(1),
+                                           _lib.raw_ptr(v), v.stride(0), v.stride(1), tokens,
+                                           None if rotary is None else ctypes.byref(rotary), _lib.raw_ptr(q), *strides,
+                                           ptr(q_out), stream_ptr()), 'svx_paged_append')
+    return q_out
+
+
+def paged_attention_workspace(tokens, sequences, q_heads, kv_heads, dim, device, max_query=0):
+    """Scratch of one `paged_attention` call of these sizes (for one call at a time)."""
+    with torch.cuda.device(device):
+        size = _lib.load().svx_paged_attention_workspace_bytes(tokens, sequences, q_heads, kv_heads, dim,
+                                                               int(max_query))
+    _need(size > 0, f'paged_attention does not take {q_heads} query heads over {kv_heads} of dim {dim}')
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True, scale=None, out=None, lse=None,
+                    max_query=None, workspace=None, status=None):
+    """Attention of new tokens over the keys of their sequences in a paged cache (`paged_append`'s arguments).
+
+    q [tokens, q_heads, dim] (token and head strides multiples of 8), dim 64, 96 or 128, query head h reading kv head
+    h // (q_heads / kv_heads). Sequence s's rows are its last tokens: causal, row i of n sees lengths[s] - n + i + 1 keys;
+    else all lengths[s]. A row that sees none gives 0. scale: 1 / sqrt(dim) unless given. Returns out [tokens, q_heads,
+    dim] (contiguous, not overlapping q); rows outside of every sequence are left as they were. lse [tokens, q_heads]
+    float32 (optional): the natural logarithm of the row's sum of exponentials, -inf for a row without keys.
+    max_query: the most new tokens of a sequence in the batch, where the caller knows it; it picks the kernel's form, never
+    the result's meaning. workspace: from `paged_attention_workspace`, not shared by calls that may overlap; allocated
+    here unless given. status [sequences] int32 (optional) gets STATUS_BAD_PAGE where a page id lies outside the pool (read
+    as zeros) or a length outside the table (clamped)."""
+    cache = _paged_cache(k_pages, v_pages, table, lengths, offsets, status)
+    _rows('q', q, None, None, cache.dim, k_pages.dtype)
+    tokens, heads = q.shape[:2]
+    _need(cache.dim in (64, 96, 128), f'dim must be 64, 96 or 128, got {cache.dim}')
+    _need(heads > 0 and heads % cache.kv_heads == 0,
+          f'{heads} query heads are not a multiple of the {cache.kv_heads} heads of the cache')
+    scale = cache.dim ** -0.5 if scale is None else float(scale)
+    _need(0 < scale <= 1e30, 'scale must be positive and finite')
+    if out is None:
+        out = torch.empty((tokens, heads, cache.dim), device=q.device, dtype=q.dtype)
+    else:
+        _rows('out', out, tokens, heads, cache.dim, q.dtype)
+    _need(lse is None or (tuple(lse.shape) == (tokens, heads) and lse.dtype == torch.float32),
+          f'lse must be a float32 [{tokens}, {heads}] tensor')
+    _need(max_query is None or max_query >= 0, 'max_query must not be negative')
+    _no_grad(q, k_pages, v_pages)
+    limit = 0 if max_query is None else min(int(max_query), 2 ** 31 - 1)
+    device = _device_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
+    with torch.cuda.device(device):
+        lib = _lib.load()
+        size = lib.svx_paged_attention_workspace_bytes(tokens, cache.sequences, heads, cache.kv_heads, cache.dim, limit)
+        if workspace is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        _need(workspace.dtype == torch.uint8 and workspace.numel() >= size,
+              f'workspace must be a uint8 tensor of at least {size} bytes')
+        check(lib.svx_paged_attention(ctypes.byref(cache), _lib.raw_ptr(q), q.stride(0), q.stride(1), tokens, heads,
+                                      int(causal), scale, ptr(out), ptr(lse), limit, ptr(workspace), stream_ptr()),
+              'svx_paged_attention')
     return out
