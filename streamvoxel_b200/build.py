@@ -19,7 +19,8 @@ ROOT = os.path.dirname(PACKAGE)
 CSRC = os.path.join(PACKAGE, 'csrc')
 BUILD = os.path.join(PACKAGE, '_build')
 LIBRARY = os.path.join(PACKAGE, 'libsvx.so')
-SOURCES = ['capi.cu', 'ease.cu', 'gemm.cu', 'attention.cu', 'embed_norm.cu', 'engine.cu', 'rope.cu', 'paged.cu']
+SOURCES = ['capi.cu', 'ease.cu', 'gemm.cu', 'attention.cu', 'embed_norm.cu', 'engine.cu', 'rope.cu', 'paged.cu',
+           'paged_tc.cu']
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 FLAGS = ['-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC', '-Xcompiler', '-fvisibility=hidden',
          '-I' + os.path.join(ROOT, 'include')]

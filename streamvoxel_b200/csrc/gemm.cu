@@ -801,14 +801,14 @@ static int make_kmajor_map(CUtensorMap* map, const void* ptr, int rows, int cols
 
 int make_map_3d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t groups, uint64_t rows,
                 uint64_t group_stride_bytes, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_rows,
-                CUtensorMapSwizzle swizzle) {
+                CUtensorMapSwizzle swizzle, uint32_t box_groups) {
   EncodeTiled encode = encode_fn();
   if (!encode) return fail(SVX_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   SVX_REQUIRE((reinterpret_cast<uintptr_t>(ptr) & 15u) == 0, "TMA operand must be 16-byte aligned");
   SVX_REQUIRE(group_stride_bytes % 16 == 0 && row_stride_bytes % 16 == 0, "TMA strides must be multiples of 16 bytes");
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)groups, (cuuint64_t)rows};
   cuuint64_t strides[2] = {(cuuint64_t)group_stride_bytes, (cuuint64_t)row_stride_bytes};
-  cuuint32_t box[3] = {box_inner, 1, box_rows};
+  cuuint32_t box[3] = {box_inner, box_groups, box_rows};
   cuuint32_t elem[3] = {1, 1, 1};
   CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, elem,
                       CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1045,5 +1045,5 @@ extern "C" int svx_gemm_group(const uint16_t* A0, const uint16_t* W0, uint16_t* 
 extern "C" uint32_t svx_wait_timeouts(void) {
   uint32_t v = 0;
   if (cudaMemcpyFromSymbol(&v, g_svx_timeouts, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
-  return v | attention_timeouts();
+  return v | attention_timeouts() | paged_timeouts();
 }

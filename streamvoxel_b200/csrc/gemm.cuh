@@ -43,8 +43,9 @@ int gemm_run_group(const GemmPlan& p0, uint16_t* out0, const EpiParams& e0, cons
 // (box_inner 32); elements past `inner` read 0.
 int make_map_3d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t groups, uint64_t rows,
                 uint64_t group_stride_bytes, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_rows,
-                CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+                CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, uint32_t box_groups = 1);
 uint32_t attention_timeouts();
+uint32_t paged_timeouts();
 int epi_from_args(const svx_epilogue_args* e, EpiParams* ep, int N, int K);
 int attention_run(const uint16_t* q, int64_t q_row_stride, const uint16_t* k, const uint16_t* v,
                   int64_t kv_slot_stride, int64_t kv_head_stride, int64_t kv_row_stride, const int32_t* lengths,

@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
   }
 }
 
-// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, rows
-// 4 y to 4 y + 3, two warps a row that share its parts.
+// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, four rows
+// at a time from 4 y on, two warps a row that share its parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   grid_dependency_wait();
@@ -384,60 +384,64 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   __shared__ float2 s_ml[8];
   Cursor at;
   at.set(p, join.s, join.j, join.h);
-  const int warp = warp_id(), lane = lane_id(), r = blockIdx.y * 4 + warp / 2, c = blockIdx.x;
+  const int warp = warp_id(), lane = lane_id(), c = blockIdx.x;
   const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
   const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
-  const bool live = r < tokens * part;
   const int parts = c - join.first + 1;
   auto slot = [&](int i) { return 2 * (join.first + i) + (i == 0 ? join.first_slot : 0); };
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, total = 0.f;
-  if (live) {
-    for (int i0 = warp & 1; i0 < parts; i0 += 64) {
-      const int i = i0 + 2 * lane;   // this warp's parts: every second one
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (i < parts) ml = p.partial_ml[(int64_t)slot(i) * p.rows + r];
-      float now = ml.x;
+  for (int r0 = blockIdx.y * 4; r0 < p.rows; r0 += gridDim.y * 4) {
+    const int r = r0 + warp / 2, in_tile = r % p.tile_rows, token = r / p.tile_rows * p.tile_tokens + in_tile / part;
+    const bool live = in_tile < p.tile_tokens * part && token < tokens;
+    if (!__syncthreads_or(live)) continue;   // also: the last round's shared values have been read
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, total = 0.f;
+    if (live) {
+      for (int i0 = warp & 1; i0 < parts; i0 += 64) {
+        const int i = i0 + 2 * lane;   // this warp's parts: every second one
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (i < parts) ml = p.partial_ml[(int64_t)slot(i) * p.rows + r];
+        float now = ml.x;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-      now = fmaxf(now, top);
-      const float old = top == now ? 1.f : exp2_approx(top - now);
-      const float f = ml.x == now ? 1.f : exp2_approx(ml.x - now);
-      float add = ml.y * f;
+        for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+        now = fmaxf(now, top);
+        const float old = top == now ? 1.f : exp2_approx(top - now);
+        const float f = ml.x == now ? 1.f : exp2_approx(ml.x - now);
+        float add = ml.y * f;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-      total = total * old + add;
-      sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
-      top = now;
-      const int here = min(32, (parts - i0 + 1) / 2);
+        for (int d = 16; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+        total = total * old + add;
+        sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+        top = now;
+        const int here = min(32, (parts - i0 + 1) / 2);
 #pragma unroll 8
-      for (int x = 0; x < here; ++x) {
-        const float fx = __shfl_sync(0xffffffffu, f, x);
-        if (lane < D / 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.partial_o + ((int64_t)slot(i0 + 2 * x) * p.rows + r) * D + 4 * lane);
-          sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
-          sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
+        for (int x = 0; x < here; ++x) {
+          const float fx = __shfl_sync(0xffffffffu, f, x);
+          if (lane < D / 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p.partial_o + ((int64_t)slot(i0 + 2 * x) * p.rows + r) * D + 4 * lane);
+            sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
+            sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
+          }
         }
       }
     }
+    s_o[warp][lane] = sum;
+    if (lane == 0) s_ml[warp] = make_float2(top, total);
+    __syncthreads();
+    if (!live || (warp & 1)) continue;
+    const float2 other = s_ml[warp + 1];
+    const float4 v = s_o[warp + 1][lane];
+    const float now = fmaxf(top, other.x);
+    const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
+    total = total * f + other.y * g;
+    const float inverse = total == 0.f ? 0.f : 1.f / total;
+    const int64_t out_row = (int64_t)(at.q.row0 + token0 + token) * p.q_heads + at.h / p.blocks * p.group + g0 + in_tile % part;
+    if (lane < D / 4)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
+          make_uint2(Half<T>::pack((sum.x * f + v.x * g) * inverse, (sum.y * f + v.y * g) * inverse),
+                     Half<T>::pack((sum.z * f + v.z * g) * inverse, (sum.w * f + v.w * g) * inverse));
+    if (lane == 0 && p.lse)
+      p.lse[out_row] = total == 0.f ? -INFINITY : (now - Half<T>::shift + log2f(total)) * 0.69314718056f;
   }
-  s_o[warp][lane] = sum;
-  if (lane == 0) s_ml[warp] = make_float2(top, total);
-  __syncthreads();
-  if (!live || (warp & 1)) return;
-  const float2 other = s_ml[warp + 1];
-  const float4 v = s_o[warp + 1][lane];
-  const float now = fmaxf(top, other.x);
-  const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
-  total = total * f + other.y * g;
-  const float inverse = total == 0.f ? 0.f : 1.f / total;
-  const int64_t out_row = (int64_t)(at.q.row0 + token0 + r / part) * p.q_heads + at.h / p.blocks * p.group + g0 + r % part;
-  if (lane < D / 4)
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
-        make_uint2(Half<T>::pack((sum.x * f + v.x * g) * inverse, (sum.y * f + v.y * g) * inverse),
-                   Half<T>::pack((sum.z * f + v.z * g) * inverse, (sum.w * f + v.w * g) * inverse));
-  if (lane == 0 && p.lse)
-    p.lse[out_row] = total == 0.f ? -INFINITY : (now - Half<T>::shift + log2f(total)) * 0.69314718056f;
 }
 
 int sm_count(int* sms) {
@@ -460,38 +464,54 @@ int few_rows_launch(const Params& p, int ctas, cudaStream_t stream) {
   return launch_dependent("few_rows_kernel", few_rows_kernel<T, D>, dim3(ctas), dim3(kThreads), Shape<D>::smem, stream, p);
 }
 
-template <typename T>
-int launch_all(const Params& p, int dim, int ctas, cudaStream_t stream) {
-  const dim3 grid(ctas, (p.rows + 3) / 4);
-  int rc;
-  if (dim == 64) rc = few_rows_launch<T, 64>(p, ctas, stream);
-  else if (dim == 96) rc = few_rows_launch<T, 96>(p, ctas, stream);
-  else rc = few_rows_launch<T, 128>(p, ctas, stream);
-  if (rc) return rc;
-  if (dim == 64) return launch_dependent("join_kernel", join_kernel<T, 64>, grid, dim3(256), 0, stream, p);
-  if (dim == 96) return launch_dependent("join_kernel", join_kernel<T, 96>, grid, dim3(256), 0, stream, p);
-  return launch_dependent("join_kernel", join_kernel<T, 128>, grid, dim3(256), 0, stream, p);
-}
-
 // How a call is divided: set from its shape alone, so that the workspace's size and the launch agree.
 struct Division {
-  int group_part, blocks, unit_tokens, rows, ctas, min_tiles;
+  bool chunk;   // the form for many rows
+  int group_part, blocks, unit_tokens, tile_tokens, tile_rows, rows, ctas, min_tiles;
 };
 
-int divide(int group, Division* d) {
+int divide(int tokens, int sequences, int group, int max_query, bool chunk_fits, Division* d) {
   int sms = 0;
   if (const int rc = sm_count(&sms)) return rc;
-  d->group_part = std::min(group, kRows);
-  d->blocks = (group + kRows - 1) / kRows;
-  d->unit_tokens = kRows / d->group_part;
-  d->rows = kRows;
-  d->ctas = sms * kCtasPerSm;
-  d->min_tiles = 2;
+  // Rows for each key: of the longest chunk where the caller knows it, else of the mean one.
+  const int64_t query = max_query > 0 ? std::min(max_query, tokens) : (tokens + sequences - 1) / std::max(sequences, 1);
+  d->chunk = chunk_fits && query * group > kRows && group <= 128;
+  if (d->chunk) {
+    d->group_part = group;
+    d->blocks = 1;
+    d->tile_tokens = 128 / group;
+    d->unit_tokens = 2 * d->tile_tokens;
+    d->tile_rows = 128;
+    d->rows = 256;
+    d->ctas = sms;
+    d->min_tiles = 4;
+  } else {
+    d->group_part = std::min(group, kRows);
+    d->blocks = (group + kRows - 1) / kRows;
+    d->unit_tokens = d->tile_tokens = kRows / d->group_part;
+    d->tile_rows = d->rows = kRows;
+    d->ctas = sms * kCtasPerSm;
+    d->min_tiles = 2;
+  }
   return SVX_OK;
 }
 
 size_t workspace_bytes(const Division& d, int dim) {
   return (size_t)d.ctas * (sizeof(Join) + 2 * (size_t)d.rows * (dim * sizeof(float) + sizeof(float2)));
+}
+
+template <typename T>
+int launch_all(const Params& p, const Division& d, int dtype, int dim, cudaStream_t stream) {
+  int rc;
+  if (d.chunk) rc = chunk_launch(p, dtype, dim, d.ctas, stream);
+  else if (dim == 64) rc = few_rows_launch<T, 64>(p, d.ctas, stream);
+  else if (dim == 96) rc = few_rows_launch<T, 96>(p, d.ctas, stream);
+  else rc = few_rows_launch<T, 128>(p, d.ctas, stream);
+  if (rc) return rc;
+  const dim3 grid(d.ctas, d.chunk ? 16 : 4);
+  if (dim == 64) return launch_dependent("join_kernel", join_kernel<T, 64>, grid, dim3(256), 0, stream, p);
+  if (dim == 96) return launch_dependent("join_kernel", join_kernel<T, 96>, grid, dim3(256), 0, stream, p);
+  return launch_dependent("join_kernel", join_kernel<T, 128>, grid, dim3(256), 0, stream, p);
 }
 
 int check_attention(int tokens, int q_heads, int kv_heads, int dim) {
@@ -510,10 +530,9 @@ using namespace svx;
 
 extern "C" size_t svx_paged_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int dim,
                                                       int max_query) {
-  (void)sequences; (void)max_query;
-  if (paged::check_attention(tokens, q_heads, kv_heads, dim)) return 0;
+  if (sequences < 0 || paged::check_attention(tokens, q_heads, kv_heads, dim)) return 0;
   paged::Division d;
-  if (paged::divide(q_heads / kv_heads, &d)) return 0;
+  if (paged::divide(tokens, sequences, q_heads / kv_heads, max_query, true, &d)) return 0;
   return paged::workspace_bytes(d, dim);
 }
 
@@ -524,15 +543,19 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   if (const int rc = check_cache(cache, "svx_paged_attention", &shift)) return rc;
   if (const int rc = paged::check_attention(tokens, q_heads, cache->kv_heads, cache->dim)) return rc;
   SVX_REQUIRE(scale > 0.f && scale <= 1e30f, "svx_paged_attention: scale must be positive and finite");
-  (void)max_query;
   if (!tokens || !cache->sequences) return SVX_OK;
   SVX_REQUIRE(q && out && workspace, "svx_paged_attention: null arguments");
+  if (tokens == 1) q_token_stride = (int64_t)q_heads * cache->dim;   // one token, one head: any stride will do
+  if (q_heads == 1) q_head_stride = cache->dim;
   SVX_REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0,
               "svx_paged_attention: strides of q must be multiples of 8 elements");
   SVX_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u) == 0,
               "svx_paged_attention: operands must be 16-byte aligned");
   paged::Division d;
-  if (const int rc = paged::divide(q_heads / cache->kv_heads, &d)) return rc;
+  // The form for many rows reads through tensor maps, whose strides are positive and whose coordinates have 32 bits; the
+  // other one takes everything, and less workspace.
+  const bool fits = q_token_stride > 0 && q_head_stride > 0 && (int64_t)cache->pages * cache->kv_heads < INT32_MAX;
+  if (const int rc = paged::divide(tokens, cache->sequences, q_heads / cache->kv_heads, max_query, fits, &d)) return rc;
   paged::Params p{};
   p.q = q;
   p.q_token = q_token_stride;
@@ -562,8 +585,11 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   p.unit_tokens = d.unit_tokens;
   p.blocks = d.blocks;
   p.group_part = d.group_part;
+  p.tile_tokens = d.tile_tokens;
+  p.tile_rows = d.tile_rows;
   p.rows = d.rows;
   p.min_tiles = d.min_tiles;
-  if (cache->dtype == SVX_BF16) return paged::launch_all<__nv_bfloat16>(p, cache->dim, d.ctas, as_stream(stream));
-  return paged::launch_all<__half>(p, cache->dim, d.ctas, as_stream(stream));
+  if (cache->dtype == SVX_BF16)
+    return paged::launch_all<__nv_bfloat16>(p, d, cache->dtype, cache->dim, as_stream(stream));
+  return paged::launch_all<__half>(p, d, cache->dtype, cache->dim, as_stream(stream));
 }

@@ -28,6 +28,7 @@ struct Params {
   int unit_tokens;           // tokens of a unit
   int blocks;                // units of one (token tile, kv head): its group in parts of at most group_part heads
   int group_part;
+  int tile_tokens, tile_rows;  // a unit's rows: tiles of tile_rows of them, tile_tokens tokens in each
   int rows;                  // rows of a partial
   int min_tiles;             // key tiles of a CTA at least
 };
@@ -204,6 +205,9 @@ struct Cursor {
 struct Join {
   int valid, s, j, h, first, first_slot, pad0, pad1;
 };
+
+// The form for many rows (paged_tc.cu).
+int chunk_launch(const Params& p, int dtype, int dim, int ctas, cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace svx

@@ -1,0 +1,578 @@
+// Attention of chunks of new tokens over a paged cache on the 5th-generation tensor cores.
+//
+// Same mathematics and the same division into equal runs of 64-key tiles as the few-rows form (paged.cu, paged.cuh), for
+// calls with many query rows for each key, which are bound by the products and the softmax's exponentials instead of
+// memory. A unit is two 128-row query tiles of one (sequence, kv head): the rows of a tile are 128 / group tokens with
+// all the query heads of the group, so that a key tile is loaded once for the whole group, and a short chunk still
+// fills the rows of the products.
+//
+// A persistent CTA per SM takes its run of the line of tiles. K and V tiles of 64 keys are streamed by TMA through
+// rings, one box per page (or 64 keys of a larger page), the page ids looked up one tile ahead. Boxes past the
+// sequence's end load nothing and come as zeros; in the box that holds the end, the rows of V past it are zeroed in
+// shared memory before the products see them, so that nothing a page holds past the length (NaN, infinities) reaches
+// 0 x v. Rows are 128 B pieces of 64 dims, 128B-swizzled, for Q, K and V alike (dims 96-127 of 96 read as zeros and
+// are not multiplied).
+//
+// Tensor memory: S_i fp32 at [64 i, +64), P_i (16-bit pairs) at [128 + 32 i, +32), O_i fp32 at [192 + 128 i, +D): S, P
+// and O of a query tile are separate, so that S_i(t+1) is computed while the softmax of tile t runs and P_i(t) V(t)
+// while it works on t + 1; 96-key tiles would not fit beside two O tiles of 128.
+//
+// Warp roles (384 threads): warp 0 loads Q and the K ring, warp 2 the V ring, warps 1 and 3 issue the products of query
+// tiles 0 and 1 (each loop warp-converged, one elected lane issuing), warps 4-7 and 8-11 run their softmax, one row a
+// thread. The exponent base is raised lazily (only when a row's maximum grows by more than 8 in log2 units), a part of
+// the exponentials is evaluated on the FMA pipe; weights are rounded to the cache's type for P V and summed unrounded.
+// A query tile without tokens (the second of a short chunk) is skipped by its chain, and a warp without live rows
+// skips the arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
+#include <math.h>
+
+#include "common.cuh"
+#include "gemm.cuh"
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace svx {
+
+__device__ uint32_t g_svx_paged_timeouts = 0;
+
+uint32_t paged_timeouts() {
+  uint32_t v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_svx_paged_timeouts, sizeof(v)) != cudaSuccess) return 0xFFFFFFFFu;
+  return v;
+}
+
+namespace paged {
+namespace {
+
+constexpr int TQ = 128, TK = kTile;
+constexpr int kThreads = 384;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 192;
+
+template <int D> struct Tiles {
+  static constexpr int atoms = (D + 63) / 64;             // 128-byte pieces of a row
+  static constexpr uint32_t q_atom = TQ * 128, q_bytes = atoms * q_atom;
+  static constexpr uint32_t k_atom = TK * 128, k_bytes = atoms * k_atom;
+  static constexpr int stages = atoms == 2 ? 5 : 10;
+  static constexpr int bars = 2 + 4 * stages + 1 + 8;
+  static constexpr size_t smem = 1024 + 2 * q_bytes + 2 * stages * k_bytes + bars * 8 + 16;
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+template <typename T> struct Kind;
+template <> struct Kind<__nv_bfloat16> {
+  static constexpr uint32_t format = 1;   // of the instruction descriptor's A and B
+  static constexpr float shift = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return tc::pack_bf16x2(lo, hi); }
+};
+template <> struct Kind<__half> {
+  static constexpr uint32_t format = 0;
+  static constexpr float shift = 7.f;     // weights are held 2^7 larger (at most 2^15 with the lazy base): see paged.cu
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+    return d;
+  }
+};
+
+// kind::f16, fp32 accumulator, A K-major, B K-major or MN-major.
+__host__ __device__ constexpr uint32_t descriptor(uint32_t format, int m, int n, bool b_mn) {
+  return (1u << 4) | (format << 7) | (format << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+// Warp-collective: `Steps` products over 16 of K each, both operands K-major in one 128B-swizzled atom (a step is 32
+// bytes, +2 in descriptor units). acc = 0: the first one starts D afresh.
+template <int Steps>
+__device__ __forceinline__ void mma_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  static_assert(Steps == 2 || Steps == 4, "steps of an atom");
+  if constexpr (Steps == 4) {
+    asm volatile(
+        "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p0;\n\t"
+        "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t"
+        "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t"
+        "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p0;\n\t"
+        "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  }
+}
+
+// Warp-collective: O += P V over 64 keys: A = P in tensor memory (8 columns a step), B = V MN-major (16 keys x 128 B a
+// step, +128 in descriptor units).
+__device__ __forceinline__ void mma_pv_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 y;\n\t.reg .b32 x;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p0;\n\t"
+      "add.s32 x, %1, 8;\n\tadd.s64 y, %2, 128;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t"
+      "add.s32 x, %1, 16;\n\tadd.s64 y, %2, 256;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t"
+      "add.s32 x, %1, 24;\n\tadd.s64 y, %2, 384;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// max(a, b, c), NaN where any of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max2_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^x on the FMA pipe for a pair: x = j + f with j = rint(x) from the 1.5 * 2^23 magic sum, a degree-4 polynomial fitted
+// to 2^f on [-0.5, 0.5] (relative error 2.7e-6), j added to the exponent field; x is clamped at -125.5.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -125.5f);
+  x.y = fmaxf(x.y, -125.5f);
+  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
+  const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(j, make_float2(-1.f, -1.f), x);
+  float2 q = __ffma2_rn(make_float2(0.009570068679749966f, 0.009570068679749966f), f,
+                        make_float2(0.055917806923389435f, 0.055917806923389435f));
+  q = __ffma2_rn(q, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  q = __ffma2_rn(q, f, make_float2(0.6931218504905701f, 0.6931218504905701f));
+  q = __ffma2_rn(q, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+
+// Of every 8 pairs of exponentials, this many go to the FMA pipe.
+constexpr int kPolyPairs = 2;
+
+// A CTA's run, unit by unit: key tiles [t0, t1) of the unit at `at`.
+struct Walk {
+  Cursor at;
+  int t0, t1, left, units;
+  __device__ __forceinline__ Walk(const Params& p, const Place& place) {
+    left = (int)(place.end - place.begin);
+    units = 0;
+    if (left <= 0) return;
+    at.set(p, place.s, place.j, place.h);
+    t0 = place.t;
+    t1 = min(at.tiles, t0 + left);
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void next(const Params& p) {
+    left -= t1 - t0;
+    ++units;
+    if (left <= 0) return;
+    at.next(p);
+    t0 = 0;
+    t1 = min(at.tiles, left);
+  }
+};
+
+// Live query tiles of a unit (tile_tokens tokens each).
+__device__ __forceinline__ int live_tiles(const Params& p, const Cursor& at, int tile_tokens) {
+  return at.q.n - at.j * p.unit_tokens > tile_tokens ? 2 : 1;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Maps maps, const Params p) {
+  using C = Tiles<D>;
+  using K = Kind<T>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PlanShared plan_shared;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;
+  uint8_t* sk = sq + 2 * C::q_bytes;
+  uint8_t* sv = sk + C::stages * C::k_bytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sv + C::stages * C::k_bytes);
+  uint64_t* q_empty = q_full + 1;             // both chains are past their last S of a unit
+  uint64_t* k_full = q_full + 2;
+  uint64_t* k_empty = k_full + C::stages;
+  uint64_t* v_full = k_empty + C::stages;
+  uint64_t* v_empty = v_full + C::stages;
+  uint64_t* v_end = v_empty + C::stages;      // the load of a V tile that holds the sequence's end
+  uint64_t* s_full = v_end + 1;               // per query tile: S_i computed
+  uint64_t* s_empty = s_full + 2;             // per query tile, 128 arrivals: S_i has been read
+  uint64_t* p_full = s_empty + 2;             // per query tile, 128 arrivals: P_i written (and O_i rescaled)
+  uint64_t* pv_done = p_full + 2;             // per query tile: P_i V completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + C::bars);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
+  const int tile_tokens = p.tile_tokens;
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int i = 0; i < C::stages; ++i) {
+      mbar_init(k_full + i, 1); mbar_init(k_empty + i, 2);
+      mbar_init(v_full + i, 1); mbar_init(v_empty + i, 2);
+    }
+    mbar_init(v_end, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1); mbar_init(s_empty + i, 128); mbar_init(p_full + i, 128); mbar_init(pv_done + i, 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::prefetch_map(&maps.q);
+    tc::prefetch_map(&maps.k);
+    tc::prefetch_map(&maps.v);
+  }
+  if (warp == 1) tc::tmem_alloc(tmem_slot, TMEM_COLS);
+  grid_dependency_wait();
+  plan<kThreads>(p, cta, gridDim.x, plan_shared);
+  if (threadIdx.x == 0) reinterpret_cast<Join*>(p.join)[cta].valid = 0;
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Place& place = plan_shared.place;
+  const int page_mask = (1 << p.page_shift) - 1, box = min(TK, 1 << p.page_shift), boxes = TK / box;
+  const int nowhere = p.pages * p.kv_heads;   // a coordinate past the pool: loads zeros
+
+  if (warp < 4) {
+    if (warp == 0 || warp == 2) {   // K with Q, and V
+      const bool is_v = warp == 2;
+      uint64_t* full = is_v ? v_full : k_full;
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      uint8_t* ring = is_v ? sv : sk;
+      const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+      Walk w(p, place);
+      int g = 0, ends = 0;
+      bool ok = true;
+      // The page id of box `lane` of tile t, as the pool's coordinate.
+      auto look_up = [&](const Cursor& at, int t) {
+        const int key = t * TK + lane * box;
+        int z = nowhere;
+        if (lane < boxes && key < at.limit) {
+          const int id = __ldg(p.table + (int64_t)at.s * p.table_width + (key >> p.page_shift));
+          if (id >= 0 && id < p.pages) z = id * p.kv_heads + at.h;
+          else if (!is_v && p.status) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
+        }
+        return z;
+      };
+      int z = w.more() ? look_up(w.at, w.t0) : nowhere;
+      while (ok && w.more()) {
+        if (!is_v) {
+          if (w.units && !tc::wait_w(q_empty, (w.units - 1) & 1, abort_flag)) { ok = false; break; }
+          const int nq = live_tiles(p, w.at, tile_tokens);
+          const uint32_t tile_bytes = C::atoms * 128 * tile_tokens * p.group;
+          tc::expect_tx_w(q_full, nq * tile_bytes);
+          for (int i = 0; i < nq; ++i)
+            for (int a = 0; a < C::atoms; ++a)
+              tc::tma_load_3d_w(sq + i * C::q_bytes + a * C::q_atom, &maps.q, a * 64, w.at.h * p.group,
+                                w.at.q.row0 + w.at.j * p.unit_tokens + i * tile_tokens, q_full);
+        }
+        const Cursor at = w.at;
+        const int t0 = w.t0, t1 = w.t1;
+        w.next(p);
+        for (int t = t0; t < t1; ++t, ++g) {
+          const int s = g % C::stages;
+          if (g >= C::stages && !tc::wait_w(empty + s, (g / C::stages - 1) & 1, abort_flag)) { ok = false; break; }
+          const int left = at.q.len - t * TK;   // keys of the sequence from this tile on
+          const bool end = is_v && left > 0 && left < TK && left % box != 0;
+          uint64_t* bar = end ? v_end : full + s;
+          uint8_t* dst = ring + s * C::k_bytes;
+          tc::expect_tx_w(bar, C::k_bytes);
+          for (int b = 0; b < boxes; ++b) {
+            const int zb = __shfl_sync(0xffffffffu, z, b), row = (t * TK + b * box) & page_mask;
+            for (int a = 0; a < C::atoms; ++a)
+              tc::tma_load_3d_w(dst + a * C::k_atom + b * box * 128, map, a * 64, zb, row, bar);
+          }
+          if (end) {   // rows past the end may hold anything: zeros, then the tile is complete
+            if (!tc::wait_w(v_end, ends & 1, abort_flag)) { ok = false; break; }
+            ++ends;
+            const int rows = box - left % box;   // to the end of the box
+            for (int e = lane; e < C::atoms * rows * 8; e += 32) {
+              const int a = e / (rows * 8), r = e % (rows * 8);
+              *reinterpret_cast<uint4*>(dst + a * C::k_atom + left * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(full + s);
+          }
+          if (t + 1 < t1) z = look_up(at, t + 1);
+          else if (w.more()) z = look_up(w.at, w.t0);
+        }
+      }
+      if (!ok)   // loads in flight end before the block does
+        for (int u = max(0, g - C::stages); u < g; ++u) mbar_wait(full + u % C::stages, (u / C::stages) & 1);
+    } else {   // warp 1: products of query tile 0; warp 3: of query tile 1
+      const int i = warp == 1 ? 0 : 1;
+      constexpr uint32_t idesc_s = descriptor(K::format, TQ, TK, false);
+      constexpr uint32_t idesc_o = descriptor(K::format, TQ, D, true);
+      const uint32_t qa = smem_addr(sq + i * C::q_bytes);
+      const uint32_t s_tmem = tmem + S_COL + 64 * i, p_tmem = tmem + P_COL + 32 * i, o_tmem = tmem + O_COL + 128 * i;
+      int g0 = 0, n0 = 0;   // tiles of the ring, and of this chain, before the unit
+      bool ok = true;
+      for (Walk w(p, place); ok && w.more(); w.next(p)) {
+        const int tiles = w.t1 - w.t0;
+        if (i >= live_tiles(p, w.at, tile_tokens)) {   // no rows: hand the tiles back
+          for (int t = 0; ok && t < tiles; ++t) {
+            const int g = g0 + t, s = g % C::stages;
+            ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
+            if (ok && lane == 0) tc::mbar_arrive(k_empty + s);
+            ok = ok && tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
+            if (ok && lane == 0) tc::mbar_arrive(v_empty + s);
+          }
+          if (ok && lane == 0) tc::mbar_arrive(q_empty);
+          g0 += tiles;
+          continue;
+        }
+        if (!tc::wait_w(q_full, w.units & 1, abort_flag)) break;
+        for (int t = 0; t <= tiles; ++t) {
+          if (t < tiles) {   // S(t): its K tile has landed and the softmax has read S(t - 1)
+            const int g = g0 + t, n = n0 + t, s = g % C::stages;
+            ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag) &&
+                 (n == 0 || tc::wait_w(s_empty + i, (n - 1) & 1, abort_flag));
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t kb = smem_addr(sk + s * C::k_bytes);
+            mma_ss_w<4>(s_tmem, tc::sw128_desc(qa), tc::sw128_desc(kb), idesc_s, 0u);
+            if constexpr (D > 64)
+              mma_ss_w<(D - 64) / 16>(s_tmem, tc::sw128_desc(qa + C::q_atom), tc::sw128_desc(kb + C::k_atom), idesc_s, 1u);
+            tc::commit_w(s_full + i);
+            tc::commit_w(k_empty + s);
+            if (t == tiles - 1) tc::commit_w(q_empty);
+          }
+          if (t >= 1) {   // O += P(t - 1) V(t - 1); the unit's first product starts O afresh
+            const int g = g0 + t - 1, n = n0 + t - 1, s = g % C::stages;
+            ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag) && tc::wait_w(p_full + i, n & 1, abort_flag);
+            if (!ok) break;
+            tc::fence_after();
+            mma_pv_w(o_tmem, p_tmem, tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc_o,
+                     t > 1 ? 1u : 0u);
+            tc::commit_w(pv_done + i);
+            tc::commit_w(v_empty + s);
+          }
+        }
+        g0 += tiles;
+        n0 += tiles;
+      }
+    }
+    // Teardown: the TMEM owner frees the columns once all 12 warps are past their last TMEM access.
+    tc::fence_before();
+    __syncwarp();
+    asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
+    if (warp == 1) {
+      tc::fence_after();
+      tc::tmem_dealloc(*tmem_slot, TMEM_COLS);
+    }
+    return;
+  }
+
+  const int i = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+  const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+  const uint32_t ts = tmem + lanes + S_COL + 64 * i, tp = tmem + lanes + P_COL + 32 * i,
+                 to = tmem + lanes + O_COL + 128 * i;
+  const float sl2 = p.scale_log2;
+  const int my_token = i * tile_tokens + row / p.group;
+  const bool in_tile = row < tile_tokens * p.group;
+  int n0 = 0, unit = 0;
+  bool ok = true;
+  Walk w(p, place);
+  for (; ok && w.more(); w.next(p), ++unit) {
+    const Cursor& at = w.at;
+    if (p.status && threadIdx.x == 128) {
+      if (__ldg(p.lengths + at.s) != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
+    }
+    if (i >= live_tiles(p, at, tile_tokens)) continue;
+    const int tiles = w.t1 - w.t0, token = at.j * p.unit_tokens + my_token;
+    const bool live = in_tile && token < at.q.n;
+    // Keys that this row sees; a dead row's result is not stored.
+    const int limit = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token + 1)) : at.q.len;
+    const int least = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
+    const bool warp_live = least != 0x7fffffff;
+    float m_used = -INFINITY, l_run = 0.f;
+    for (int t = 0; t < tiles; ++t) {
+      const int n = n0 + t;
+      if (!tc::wait(s_full + i, n & 1, abort_flag)) { ok = false; break; }
+      if (!warp_live) {
+        tc::mbar_arrive(s_empty + i);
+        if (n >= 1 && !tc::wait(pv_done + i, (n - 1) & 1, abort_flag)) { ok = false; break; }
+        tc::mbar_arrive(p_full + i);
+        continue;
+      }
+      tc::fence_after();
+      uint32_t r[2][32];
+      tc::ld32(ts, r[0]);
+      tc::ld32(ts + 32, r[1]);
+      tc::wait_ld();
+      tc::fence_before();
+      tc::mbar_arrive(s_empty + i);   // S_i(t + 1) may now be computed into the same columns
+      const int key0 = (w.t0 + t) * TK;
+      if (key0 + TK > least) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (key0 + c * 32 + j >= limit) r[c][j] = __float_as_uint(-INFINITY);
+      }
+      float mc[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float a = __uint_as_float(r[c][0]), b = __uint_as_float(r[c][1]);
+#pragma unroll
+        for (int j = 2; j < 30; j += 4) {
+          a = max3_nan(a, __uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1]));
+          b = max3_nan(b, __uint_as_float(r[c][j + 2]), __uint_as_float(r[c][j + 3]));
+        }
+        mc[c] = max3_nan(a, max2_nan(b, __uint_as_float(r[c][30])), __uint_as_float(r[c][31]));
+      }
+      const float mx = max2_nan(mc[0], mc[1]) * sl2;
+      // Raise the exponent base only when the row's maximum outgrows it by more than 8 (warp-uniform rescale of O). A
+      // NaN raises it too and stays: every weight of the row is NaN from then on.
+      const bool raise = !(mx <= m_used + 8.f);
+      const bool any_raise = __any_sync(0xffffffffu, raise);
+      float alpha = 1.f;
+      if (any_raise) {
+        const float m_new = raise ? mx : m_used;
+        alpha = m_used == m_new ? 1.f : tc::ex2(m_used - m_new);   // m_used = -inf: 0
+        m_used = m_new;
+      }
+      const float base = m_used == -INFINITY ? 0.f : m_used - K::shift;
+      const float2 scale2 = make_float2(sl2, sl2), nbase2 = make_float2(-base, -base);
+      float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t packed[32];
+#pragma unroll
+      for (int j = 0; j < TK; j += 2) {
+        const int c = j >> 5, jj = j & 31;
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][jj]), __uint_as_float(r[c][jj + 1])), scale2, nbase2);
+        const float2 e = ((j >> 1) & 7) < kPolyPairs ? exp2_poly(x) : make_float2(tc::ex2(x.x), tc::ex2(x.y));
+        acc[(j >> 1) & 3] = __fadd2_rn(acc[(j >> 1) & 3], e);
+        packed[j >> 1] = K::pack(e.x, e.y);
+      }
+      // P_i(t - 1) V(t - 1) has completed: P_i may be overwritten and O_i holds the products of earlier tiles.
+      if (n >= 1 && !tc::wait(pv_done + i, (n - 1) & 1, abort_flag)) { ok = false; break; }
+      tc::fence_after();
+      if (any_raise && t >= 1) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tc::ld32(to + c * 32, o);
+          tc::wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+          tc::st32(to + c * 32, o);
+        }
+      }
+      tc::st32(tp, packed);
+      tc::wait_st();
+      const float2 s01 = __fadd2_rn(acc[0], acc[1]), s23 = __fadd2_rn(acc[2], acc[3]);
+      l_run = l_run * alpha + ((s01.x + s01.y) + (s23.x + s23.y));
+      tc::fence_before();
+      tc::mbar_arrive(p_full + i);
+    }
+    if (ok) ok = tc::wait(pv_done + i, (n0 + tiles - 1) & 1, abort_flag);
+    if (!ok) break;
+    tc::fence_after();
+    n0 += tiles;
+    const bool whole = w.t0 == 0 && w.t1 == at.tiles;
+    const int64_t slot = (int64_t)(2 * cta + (unit ? 1 : 0)) * p.rows + i * TQ + row;
+    const int64_t out_row = (int64_t)(at.q.row0 + token) * p.q_heads + at.h * p.group + row % p.group;
+    // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
+    // makes the row NaN, as inf - inf does.
+    const bool none = m_used == -INFINITY;
+    if (m_used == INFINITY) l_run = __int_as_float(0x7fffffff);
+    if (none) l_run = 0.f;
+    const float factor = none ? 0.f : whole ? 1.f / l_run : 1.f;
+    if (warp_live) {
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tc::ld32(to + c * 32, o);
+        tc::wait_ld();
+        if (!live) continue;
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = none ? 0.f : __uint_as_float(o[j]) * factor;
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c * 32);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            dst[k] = make_uint4(K::pack(f[8 * k], f[8 * k + 1]), K::pack(f[8 * k + 2], f[8 * k + 3]),
+                                K::pack(f[8 * k + 4], f[8 * k + 5]), K::pack(f[8 * k + 6], f[8 * k + 7]));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.partial_o + slot * D + c * 32);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+        }
+      }
+      if (live && !whole) p.partial_ml[slot] = make_float2(m_used, l_run);
+      if (live && whole && p.lse)
+        p.lse[out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
+    }
+    if (threadIdx.x == 128 && unit == 0 && !whole && w.t1 == at.tiles) {
+      Join* join = reinterpret_cast<Join*>(p.join) + cta;
+      const int64_t first = place.unit / place.each;
+      join->s = at.s;
+      join->j = at.j;
+      join->h = at.h;
+      join->first = (int)first;
+      join->first_slot = place.unit == first * place.each ? 0 : 1;
+      join->valid = 1;
+    }
+    // O_i has been read; the next unit's first P V, which overwrites it, is issued only after this warpgroup's next
+    // p_full arrival.
+    tc::fence_before();
+  }
+  if (!ok && lane == 0) {
+    atomicOr(&g_svx_paged_timeouts, SVX_STATUS_WAIT_TIMEOUT);
+    if (p.status) atomicOr(p.status + w.at.s, SVX_STATUS_WAIT_TIMEOUT);
+  }
+  tc::fence_before();
+  __syncwarp();
+  asm volatile("barrier.arrive 1, %0;" ::"n"(kThreads) : "memory");
+}
+
+template <typename T, int D>
+int launch(const Maps& maps, const Params& p, int ctas, cudaStream_t stream) {
+  static PerDevice<int> ready;
+  int unused;
+  const int rc = ready.get(&unused, [](int, int*) -> int {
+    SVX_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tiles<D>::smem));
+    return SVX_OK;
+  });
+  if (rc) return rc;
+  return launch_dependent("chunk_kernel", chunk_kernel<T, D>, dim3(ctas), dim3(kThreads), Tiles<D>::smem, stream, maps, p);
+}
+
+}  // namespace
+
+int chunk_launch(const Params& p, int dtype, int dim, int ctas, cudaStream_t stream) {
+  Maps maps;
+  const int page = 1 << p.page_shift, box = page < TK ? page : TK, tile_tokens = p.tile_tokens;
+  const uint64_t pools = (uint64_t)p.pages * p.kv_heads;
+  int rc = make_map_3d(&maps.q, p.q, dim, p.q_heads, p.tokens, p.q_head * 2, p.q_token * 2, 64, tile_tokens,
+                       CU_TENSOR_MAP_SWIZZLE_128B, p.group);
+  if (!rc) rc = make_map_3d(&maps.k, p.k, dim, pools, page, (uint64_t)page * dim * 2, dim * 2, 64, box);
+  if (!rc) rc = make_map_3d(&maps.v, p.v, dim, pools, page, (uint64_t)page * dim * 2, dim * 2, 64, box);
+  if (rc) return rc;
+  if (dtype == SVX_BF16) {
+    if (dim == 64) return launch<__nv_bfloat16, 64>(maps, p, ctas, stream);
+    if (dim == 96) return launch<__nv_bfloat16, 96>(maps, p, ctas, stream);
+    return launch<__nv_bfloat16, 128>(maps, p, ctas, stream);
+  }
+  if (dim == 64) return launch<__half, 64>(maps, p, ctas, stream);
+  if (dim == 96) return launch<__half, 96>(maps, p, ctas, stream);
+  return launch<__half, 128>(maps, p, ctas, stream);
+}
+
+}  // namespace paged
+}  // namespace svx
