@@ -326,39 +326,70 @@ def _need(ok, text):
         raise ValueError(text)
 
 
-def _device_of(*tensors):
+# The wrappers below are called once or twice a layer for a handful of tokens, where the time of a call is the host's: they
+# read each attribute once, build their messages only when they raise, and pass plain addresses.
+
+def _launch_on(index, function, *args):
+    """function(*args, stream) on the current stream of CUDA device `index`, with that device current."""
+    if index == torch.cuda.current_device():
+        return function(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return function(*args, _raw_stream(index))
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', _raw_stream)
+
+
+def _index_of(first, *others):
     """The one CUDA device of the tensors (None entries apart)."""
-    devices = {t.device for t in tensors if t is not None}
-    _need(len(devices) == 1 and next(iter(devices)).type == 'cuda', 'operands must be on one CUDA device')
-    return devices.pop()
+    index = first.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in others):
+        raise ValueError('operands must be on one CUDA device')
+    return index
 
 
-def _rows(name, t, tokens=None, heads=None, dim=None, dtype=None):
-    """A [tokens, heads, dim] operand with contiguous rows; the token and head strides are free."""
-    _need(t.ndim == 3, f'{name} must be [tokens, heads, dim]')
-    for size, want, what in zip(t.shape, (tokens, heads, dim), ('tokens', 'heads', 'dim')):
-        _need(want is None or size == want, f'{name} has {size} {what}, expected {want}')
-    _need(dtype is None or t.dtype == dtype, f'{name} must be {dtype}')
-    _need(t.stride(2) == 1 or t.shape[2] == 1, f'{name} must have contiguous rows (stride 1 in dim)')
+def _rows(name, t, tokens, heads, dim, dtype):
+    """(token stride, head stride) of a [tokens, heads, dim] operand with contiguous rows."""
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f'{name} must be [tokens, heads, dim]')
+    if shape[0] != tokens or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f'{name} is {tuple(shape)}, expected {(tokens, heads, dim)}')
+    if t.dtype != dtype:
+        raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
+    strides = t.stride()
+    if strides[2] != 1 and dim != 1:
+        raise ValueError(f'{name} must have contiguous rows (stride 1 in dim)')
+    return strides[0], strides[1]
 
 
 def _rotary(inv_freq, positions, tokens, dim, layout, scale):
-    _need(inv_freq.dtype == torch.float64 and inv_freq.ndim == 1 and inv_freq.is_contiguous(),
-          'inv_freq must be a contiguous float64 vector, one entry per pair')
+    if inv_freq.dtype != torch.float64 or inv_freq.ndim != 1 or not inv_freq.is_contiguous():
+        raise ValueError('inv_freq must be a contiguous float64 vector, one entry per pair')
     pairs = inv_freq.numel()
-    _need(0 < 2 * pairs <= dim, f'{pairs} pairs do not fit heads of {dim}')
-    _need(layout in _lib.ROPE_LAYOUTS, f'layout must be one of {sorted(_lib.ROPE_LAYOUTS)}')
-    axes, kind = 1, _lib.I64
-    if positions is not None:
-        _need(positions.dtype in _POSITION_DTYPES, 'positions must be int32, int64 or float32')
-        _need(positions.ndim in (1, 2) and positions.shape[0] == tokens and positions.is_contiguous(),
-              f'positions must be a contiguous [{tokens}] or [{tokens}, axes] tensor')
-        axes = positions.shape[1] if positions.ndim == 2 else 1
-        kind = _POSITION_DTYPES[positions.dtype]
-        _need(axes > 0 and pairs % axes == 0, f'{axes} axes do not share {pairs} pairs evenly')
-    _need(math.isfinite(scale), 'the rotary scale must be finite')
-    return _lib.Rotary(inv_freq.data_ptr(), 2 * pairs, _lib.ROPE_LAYOUTS[layout], axes, float(scale),
-                       ptr(positions), kind)
+    if not 0 < 2 * pairs <= dim:
+        raise ValueError(f'{pairs} pairs do not fit heads of {dim}')
+    if layout not in _lib.ROPE_LAYOUTS:
+        raise ValueError(f'layout must be one of {sorted(_lib.ROPE_LAYOUTS)}')
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError('the rotary scale must be finite')
+    if positions is None:
+        return _lib.Rotary(inv_freq.data_ptr(), 2 * pairs, _lib.ROPE_LAYOUTS[layout], 1, scale, None, _lib.I64)
+    shape = positions.shape
+    if positions.dtype not in _POSITION_DTYPES:
+        raise ValueError('positions must be int32, int64 or float32')
+    if len(shape) not in (1, 2) or shape[0] != tokens or not positions.is_contiguous():
+        raise ValueError(f'positions must be a contiguous [{tokens}] or [{tokens}, axes] tensor')
+    axes = shape[1] if len(shape) == 2 else 1
+    if axes < 1 or pairs % axes:
+        raise ValueError(f'{axes} axes do not share {pairs} pairs evenly')
+    return _lib.Rotary(inv_freq.data_ptr(), 2 * pairs, _lib.ROPE_LAYOUTS[layout], axes, scale, positions.data_ptr(),
+                       _POSITION_DTYPES[positions.dtype])
 
 
 def rope_frequencies(rot, base=10000.0, *, axes=1, scaling=None, factor=1.0, original=8192, device='cuda'):
@@ -394,7 +425,7 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         layout, scale, inverse = ctx.args
-        grad = grad if grad.stride(-1) == 1 else grad.contiguous()
+        grad = grad if grad.stride(-1) == 1 else grad.contiguous()   # one broadcast over the values of a head
         return rope(grad, *ctx.saved_tensors, layout=layout, scale=scale, inverse=not inverse), *[None] * 5
 
 
@@ -406,47 +437,69 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
     float64, from `rope_frequencies`. Pairs are (2j, 2j + 1) ('interleaved') or (j, j + rot / 2) ('half'). inverse: the
     transposed rotation, the gradient's way back; x that requires grad takes it by itself. out: a [tokens, heads, dim]
     tensor of x's type, x itself or one that does not overlap it."""
-    _rows('x', x)
-    _need(x.dtype in _ROW_DTYPES, f'x must be fp32, bf16 or fp16, got {x.dtype}')
+    if x.ndim != 3:
+        raise ValueError('x must be [tokens, heads, dim]')
     tokens, heads, dim = x.shape
-    _need(heads > 0 and dim > 0, 'x has no heads or values')
-    _need(positions is not None, 'rope needs positions')
+    dtype = x.dtype
+    if dtype not in _ROW_DTYPES:
+        raise ValueError(f'x must be fp32, bf16 or fp16, got {dtype}')
+    if heads < 1 or dim < 1:
+        raise ValueError('x has no heads or values')
+    if positions is None:
+        raise ValueError('rope needs positions')
+    strides = _rows('x', x, tokens, heads, dim, dtype)
     rotary = _rotary(inv_freq, positions, tokens, dim, layout, scale)
-    if torch.is_grad_enabled() and x.requires_grad:
-        _need(out is None, 'out is not available for x that requires grad')
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError('out is not available for x that requires grad')
         return _Rope.apply(x, positions, inv_freq, layout, scale, inverse)
     if out is None:
-        out = torch.empty((tokens, heads, dim), device=x.device, dtype=x.dtype)
+        index = _index_of(x, positions, inv_freq)
+        out = x.new_empty((tokens, heads, dim))
+        out_strides = heads * dim, dim
     else:
-        _rows('out', out, tokens, heads, dim, x.dtype)
-        _need(all(n == 1 or s != 0 for n, s in zip(out.shape, out.stride())), 'out must not repeat memory')
-    with torch.cuda.device(_device_of(x, positions, inv_freq, out)):
-        check(_lib.load().svx_rope(_lib.raw_ptr(x), _ROW_DTYPES[x.dtype], x.stride(0), x.stride(1), _lib.raw_ptr(out),
-                                   out.stride(0), out.stride(1), tokens, heads, dim, ctypes.byref(rotary), int(inverse),
-                                   stream_ptr()), 'svx_rope')
+        out_strides = _rows('out', out, tokens, heads, dim, dtype)
+        if (out_strides[0] == 0 and tokens > 1) or (out_strides[1] == 0 and heads > 1):
+            raise ValueError('out must not repeat memory')
+        index = _index_of(x, positions, inv_freq, out)
+    status = _launch_on(index, _lib.load().svx_rope, x.data_ptr(), _ROW_DTYPES[dtype], *strides, out.data_ptr(),
+                        *out_strides, tokens, heads, dim, ctypes.byref(rotary), bool(inverse))
+    if status:
+        check(status, 'svx_rope')
     return out
 
 
 def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
-    _need(k_pages.ndim == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
-          'k_pages and v_pages must be [pages, kv_heads, page, dim] pools of one shape and type')
-    _need(k_pages.dtype in (torch.bfloat16, torch.float16), f'the cache must be bf16 or fp16, got {k_pages.dtype}')
-    pages, heads, page, dim = k_pages.shape
-    _need(page in (16, 32, 64, 128, 256, 512, 1024), f'a page must hold 16, 32, .. 1024 keys, got {page}')
-    for name, t in (('table', table), ('lengths', lengths), ('offsets', offsets), ('status', status)):
-        _need(t is None or t.dtype == torch.int32, f'{name} must be int32')
-    _need(table.ndim == 2 and table.shape[1] > 0, 'table must be [sequences, pages of a sequence]')
-    sequences = table.shape[0]
-    _need(tuple(lengths.shape) == (sequences,), f'lengths must be [{sequences}]')
-    _need(tuple(offsets.shape) == (sequences + 1,), f'offsets must be [{sequences + 1}]')
-    _need(status is None or tuple(status.shape) == (sequences,), f'status must be [{sequences}]')
-    return _lib.PagedCache(ptr(k_pages), ptr(v_pages), _ROW_DTYPES[k_pages.dtype], pages, heads, page, dim, sequences,
-                           table.shape[1], ptr(table), ptr(lengths), ptr(offsets), ptr(status))
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or dtype != v_pages.dtype:
+        raise ValueError('k_pages and v_pages must be [pages, kv_heads, page, dim] pools of one shape and type')
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f'the cache must be bf16 or fp16, got {dtype}')
+    pages, heads, page, dim = shape
+    if page not in (16, 32, 64, 128, 256, 512, 1024):
+        raise ValueError(f'a page must hold 16, 32, .. 1024 keys, got {page}')
+    shape = table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError('table must be [sequences, pages of a sequence]')
+    sequences, width = shape
+    if lengths.ndim != 1 or len(lengths) != sequences or offsets.ndim != 1 or len(offsets) != sequences + 1:
+        raise ValueError(f'lengths must be [{sequences}] and offsets [{sequences + 1}]')
+    if not table.dtype == lengths.dtype == offsets.dtype == torch.int32:
+        raise ValueError('table, lengths and offsets must be int32')
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and table.is_contiguous() and lengths.is_contiguous()
+            and offsets.is_contiguous()):
+        raise ValueError('the pools, table, lengths and offsets must be contiguous')
+    if status is not None:
+        if tuple(status.shape) != (sequences,) or status.dtype != torch.int32 or not status.is_contiguous():
+            raise ValueError(f'status must be a contiguous int32 [{sequences}] tensor')
+        status = status.data_ptr()
+    return _lib.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _ROW_DTYPES[dtype], pages, heads, page, dim,
+                           sequences, width, table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), status)
 
 
 def _no_grad(*tensors):
-    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
-          'the paged cache takes no part in autograd: call under torch.no_grad()')
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError('the paged cache takes no part in autograd: call under torch.no_grad()')
 
 
 def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=None, positions=None,
@@ -461,27 +514,36 @@ def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=No
     contiguous). A key whose place lies outside the table, or whose page id lies outside the pool, is not stored; status
     [sequences] int32 (optional) gets STATUS_BAD_PAGE for its sequence. Two tokens given the same place race."""
     cache = _paged_cache(k_pages, v_pages, table, lengths, offsets, status)
-    _rows('k', k, None, cache.kv_heads, cache.dim, k_pages.dtype)
-    _rows('v', v, k.shape[0], cache.kv_heads, cache.dim, k_pages.dtype)
-    tokens = k.shape[0]
-    _need(inv_freq is not None or (q is None and positions is None), 'q and positions need inv_freq')
-    _need(q is not None or q_out is None, 'q_out needs q')
-    rotary = None if inv_freq is None else _rotary(inv_freq, positions, tokens, cache.dim, layout, rope_scale)
-    if q is not None:
-        _rows('q', q, tokens, None, cache.dim, k_pages.dtype)
-        _need(0 < q.shape[1] <= 4096, 'q must have 1 to 4096 heads')
-        if q_out is None:
-            q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        else:
-            _rows('q_out', q_out, tokens, q.shape[1], cache.dim, q.dtype)
+    dtype, heads, dim, tokens = k_pages.dtype, cache.kv_heads, cache.dim, len(k)
+    k_strides = _rows('k', k, tokens, heads, dim, dtype)
+    v_strides = _rows('v', v, tokens, heads, dim, dtype)
     _no_grad(k, v, k_pages, v_pages, q)
-    strides = (0, 0, 0) if q is None else (q.stride(0), q.stride(1), q.shape[1])
-    with torch.cuda.device(_device_of(k, v, k_pages, v_pages, table, lengths, offsets, inv_freq, positions, q, q_out,
-                                      status)):
-        check(_lib.load().svx_paged_append(ctypes.byref(cache), _lib.raw_ptr(k), k.stride(0), k.stride(1),
-                                           _lib.raw_ptr(v), v.stride(0), v.stride(1), tokens,
-                                           None if rotary is None else ctypes.byref(rotary), _lib.raw_ptr(q), *strides,
-                                           ptr(q_out), stream_ptr()), 'svx_paged_append')
+    index = _index_of(k_pages, v_pages, table, lengths, offsets, k, v, inv_freq, positions, q, q_out, status)
+    rotary = None
+    if inv_freq is not None:
+        rotary = ctypes.byref(_rotary(inv_freq, positions, tokens, dim, layout, rope_scale))
+    elif q is not None or positions is not None:
+        raise ValueError('q and positions need inv_freq')
+    if q is None:
+        if q_out is not None:
+            raise ValueError('q_out needs q')
+        queries = None, 0, 0, 0, None
+    else:
+        q_heads = q.shape[1] if q.ndim == 3 else 0
+        q_strides = _rows('q', q, tokens, q_heads, dim, dtype)
+        if not 0 < q_heads <= 4096:
+            raise ValueError('q must have 1 to 4096 heads')
+        if q_out is None:
+            q_out = q.new_empty((tokens, q_heads, dim))
+        else:
+            _rows('q_out', q_out, tokens, q_heads, dim, dtype)
+            if not q_out.is_contiguous():
+                raise ValueError('q_out must be contiguous')
+        queries = q.data_ptr(), *q_strides, q_heads, q_out.data_ptr()
+    status = _launch_on(index, _lib.load().svx_paged_append, ctypes.byref(cache), k.data_ptr(), *k_strides, v.data_ptr(),
+                        *v_strides, tokens, rotary, *queries)
+    if status:
+        check(status, 'svx_paged_append')
     return q_out
 
 
@@ -508,31 +570,38 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
     here unless given. status [sequences] int32 (optional) gets STATUS_BAD_PAGE where a page id lies outside the pool (read
     as zeros) or a length outside the table (clamped)."""
     cache = _paged_cache(k_pages, v_pages, table, lengths, offsets, status)
-    _rows('q', q, None, None, cache.dim, k_pages.dtype)
-    tokens, heads = q.shape[:2]
-    _need(cache.dim in (64, 96, 128), f'dim must be 64, 96 or 128, got {cache.dim}')
-    _need(heads > 0 and heads % cache.kv_heads == 0,
-          f'{heads} query heads are not a multiple of the {cache.kv_heads} heads of the cache')
-    scale = cache.dim ** -0.5 if scale is None else float(scale)
-    _need(0 < scale <= 1e30, 'scale must be positive and finite')
-    if out is None:
-        out = torch.empty((tokens, heads, cache.dim), device=q.device, dtype=q.dtype)
-    else:
-        _rows('out', out, tokens, heads, cache.dim, q.dtype)
-    _need(lse is None or (tuple(lse.shape) == (tokens, heads) and lse.dtype == torch.float32),
-          f'lse must be a float32 [{tokens}, {heads}] tensor')
-    _need(max_query is None or max_query >= 0, 'max_query must not be negative')
+    dim, kv_heads = cache.dim, cache.kv_heads
+    tokens, heads = q.shape[:2] if q.ndim == 3 else (0, 0)
+    strides = _rows('q', q, tokens, heads, dim, k_pages.dtype)
+    if dim not in (64, 96, 128):
+        raise ValueError(f'dim must be 64, 96 or 128, got {dim}')
+    if heads < 1 or heads % kv_heads:
+        raise ValueError(f'{heads} query heads are not a multiple of the {kv_heads} heads of the cache')
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale <= 1e30:
+        raise ValueError('scale must be positive and finite')
+    if max_query is None:
+        max_query = 0
+    elif max_query < 0:
+        raise ValueError('max_query must not be negative')
     _no_grad(q, k_pages, v_pages)
-    limit = 0 if max_query is None else min(int(max_query), 2 ** 31 - 1)
-    device = _device_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
-    with torch.cuda.device(device):
-        lib = _lib.load()
-        size = lib.svx_paged_attention_workspace_bytes(tokens, cache.sequences, heads, cache.kv_heads, cache.dim, limit)
-        if workspace is None:
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        _need(workspace.dtype == torch.uint8 and workspace.numel() >= size,
-              f'workspace must be a uint8 tensor of at least {size} bytes')
-        check(lib.svx_paged_attention(ctypes.byref(cache), _lib.raw_ptr(q), q.stride(0), q.stride(1), tokens, heads,
-                                      int(causal), scale, ptr(out), ptr(lse), limit, ptr(workspace), stream_ptr()),
-              'svx_paged_attention')
+    index = _index_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
+    if out is None:
+        out = q.new_empty((tokens, heads, dim))
+    else:
+        _rows('out', out, tokens, heads, dim, q.dtype)
+        if not out.is_contiguous():
+            raise ValueError('out must be contiguous')
+    if lse is not None and (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise ValueError(f'lse must be a contiguous float32 [{tokens}, {heads}] tensor')
+    lib, max_query = _lib.load(), min(int(max_query), tokens)
+    size = lib.svx_paged_attention_workspace_bytes(tokens, cache.sequences, heads, kv_heads, dim, max_query)
+    if workspace is None:
+        workspace = q.new_empty((size,), dtype=torch.uint8)
+    elif workspace.dtype != torch.uint8 or workspace.numel() < size or not workspace.is_contiguous():
+        raise ValueError(f'workspace must be a contiguous uint8 tensor of at least {size} bytes')
+    status = _launch_on(index, lib.svx_paged_attention, ctypes.byref(cache), q.data_ptr(), *strides, tokens, heads, bool(causal),
+                        scale, out.data_ptr(), None if lse is None else lse.data_ptr(), max_query, workspace.data_ptr())
+    if status:
+        check(status, 'svx_paged_attention')
     return out
