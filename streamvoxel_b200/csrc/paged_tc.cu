@@ -13,9 +13,11 @@
 // 0 x v. Rows are 128 B pieces of 64 dims, 128B-swizzled, for Q, K and V alike (dims 96-127 of 96 read as zeros and
 // are not multiplied).
 //
-// Tensor memory: S_i fp32 at [64 i, +64), P_i (16-bit pairs) at [128 + 32 i, +32), O_i fp32 at [192 + 128 i, +D): S, P
-// and O of a query tile are separate, so that S_i(t+1) is computed while the softmax of tile t runs and P_i(t) V(t)
-// while it works on t + 1; 96-key tiles would not fit beside two O tiles of 128.
+// Tensor memory: two S buffers of each query tile (fp32, tile t in buffer t % 2 at [128 i + 64 (t % 2), +64)) and O_i
+// (fp32 at [256 + 128 i, +D)). The softmax writes P(t) (16-bit pairs) over the first 32 columns of the S buffer that it
+// has read, so S(t + 2) follows P(t) V(t) there, while S(t + 1) is ready before the softmax of tile t is done: the
+// softmax waits for no product but its own tile's. (With one S buffer and P apart the softmax waited 300-450 of the
+// 1,800 cycles of a tile for S: clock stamps.)
 //
 // Warp roles (384 threads): warp 0 loads Q and the K ring, warp 2 the V ring, warps 1 and 3 issue the products of query
 // tiles 0 and 1 (each loop warp-converged, one elected lane issuing), warps 4-7 and 8-11 run their softmax, one row a
@@ -46,14 +48,14 @@ namespace {
 constexpr int TQ = 128, TK = kTile;
 constexpr int kThreads = 384;
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t S_COL = 0, P_COL = 128, O_COL = 192;
+constexpr uint32_t S_COL = 0, O_COL = 256;   // + 128 i
 
 template <int D> struct Tiles {
   static constexpr int atoms = (D + 63) / 64;             // 128-byte pieces of a row
   static constexpr uint32_t q_atom = TQ * 128, q_bytes = atoms * q_atom;
   static constexpr uint32_t k_atom = TK * 128, k_bytes = atoms * k_atom;
   static constexpr int stages = atoms == 2 ? 5 : 10;
-  static constexpr int bars = 2 + 4 * stages + 1 + 8;
+  static constexpr int bars = 2 + 4 * stages + 1 + 12;
   static constexpr size_t smem = 1024 + 2 * q_bytes + 2 * stages * k_bytes + bars * 8 + 16;
 };
 
@@ -207,13 +209,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint64_t* v_full = k_empty + C::stages;
   uint64_t* v_empty = v_full + C::stages;
   uint64_t* v_end = v_empty + C::stages;      // the load of a V tile that holds the sequence's end
-  uint64_t* s_full = v_end + 1;               // per query tile: S_i computed
-  uint64_t* s_empty = s_full + 2;             // per query tile, 128 arrivals: S_i has been read
-  uint64_t* p_full = s_empty + 2;             // per query tile, 128 arrivals: P_i written (and O_i rescaled)
-  uint64_t* pv_done = p_full + 2;             // per query tile: P_i V completed
+  uint64_t* s_full = v_end + 1;               // per query tile and buffer: S computed
+  uint64_t* p_full = s_full + 4;              // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
+  uint64_t* pv_done = p_full + 4;             // per query tile and buffer: P V completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + C::bars);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
+  // Tile n of a chain (counted over the CTA's whole run) uses buffer n % 2, whose barriers are in phase n / 2. With one
+  // barrier for both buffers a wait could find the phase two tiles back and take it for its own.
+  auto buffer_wait = [&](uint64_t* bars, int i, int n) {
+    return tc::wait(bars + 2 * i + (n & 1), (n >> 1) & 1, abort_flag);
+  };
   const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
   const int tile_tokens = p.tile_tokens;
   grid_launch_dependents();
@@ -225,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       mbar_init(v_full + i, 1); mbar_init(v_empty + i, 2);
     }
     mbar_init(v_end, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1); mbar_init(s_empty + i, 128); mbar_init(p_full + i, 128); mbar_init(pv_done + i, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(pv_done + i, 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -318,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       constexpr uint32_t idesc_s = descriptor(K::format, TQ, TK, false);
       constexpr uint32_t idesc_o = descriptor(K::format, TQ, D, true);
       const uint32_t qa = smem_addr(sq + i * C::q_bytes);
-      const uint32_t s_tmem = tmem + S_COL + 64 * i, p_tmem = tmem + P_COL + 32 * i, o_tmem = tmem + O_COL + 128 * i;
+      const uint32_t s_tmem = tmem + S_COL + 128 * i, o_tmem = tmem + O_COL + 128 * i;
       int g0 = 0, n0 = 0;   // tiles of the ring, and of this chain, before the unit
       bool ok = true;
       for (Walk w(p, place); ok && w.more(); w.next(p)) {
@@ -336,31 +342,31 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           continue;
         }
         if (!tc::wait_w(q_full, w.units & 1, abort_flag)) break;
-        for (int t = 0; t <= tiles; ++t) {
-          if (t < tiles) {   // S(t): its K tile has landed and the softmax has read S(t - 1)
-            const int g = g0 + t, n = n0 + t, s = g % C::stages;
-            ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag) &&
-                 (n == 0 || tc::wait_w(s_empty + i, (n - 1) & 1, abort_flag));
-            if (!ok) break;
-            tc::fence_after();
-            const uint32_t kb = smem_addr(sk + s * C::k_bytes);
-            mma_ss_w<4>(s_tmem, tc::sw128_desc(qa), tc::sw128_desc(kb), idesc_s, 0u);
-            if constexpr (D > 64)
-              mma_ss_w<(D - 64) / 16>(s_tmem, tc::sw128_desc(qa + C::q_atom), tc::sw128_desc(kb + C::k_atom), idesc_s, 1u);
-            tc::commit_w(s_full + i);
-            tc::commit_w(k_empty + s);
-            if (t == tiles - 1) tc::commit_w(q_empty);
-          }
-          if (t >= 1) {   // O += P(t - 1) V(t - 1); the unit's first product starts O afresh
-            const int g = g0 + t - 1, n = n0 + t - 1, s = g % C::stages;
-            ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag) && tc::wait_w(p_full + i, n & 1, abort_flag);
-            if (!ok) break;
-            tc::fence_after();
-            mma_pv_w(o_tmem, p_tmem, tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc_o,
-                     t > 1 ? 1u : 0u);
-            tc::commit_w(pv_done + i);
-            tc::commit_w(v_empty + s);
-          }
+        auto issue_s = [&](int t) {   // S(t): its K tile has landed, and its buffer's last P V is done (the caller's wait)
+          const int g = g0 + t, s = g % C::stages;
+          if (!tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag)) return false;
+          tc::fence_after();
+          const uint32_t kb = smem_addr(sk + s * C::k_bytes), buffer = (n0 + t) & 1, d = s_tmem + 64 * buffer;
+          mma_ss_w<4>(d, tc::sw128_desc(qa), tc::sw128_desc(kb), idesc_s, 0u);
+          if constexpr (D > 64)
+            mma_ss_w<(D - 64) / 16>(d, tc::sw128_desc(qa + C::q_atom), tc::sw128_desc(kb + C::k_atom), idesc_s, 1u);
+          tc::commit_w(s_full + 2 * i + buffer);
+          tc::commit_w(k_empty + s);
+          if (t == tiles - 1) tc::commit_w(q_empty);
+          return true;
+        };
+        ok = (n0 == 0 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n0 - 1))) && issue_s(0) && (tiles == 1 || issue_s(1));
+        for (int t = 0; ok && t < tiles; ++t) {   // O += P(t) V(t), which starts O afresh first; then S(t + 2)
+          const int g = g0 + t, n = n0 + t, s = g % C::stages, buffer = n & 1;
+          ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag) &&
+               __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
+          if (!ok) break;
+          tc::fence_after();
+          mma_pv_w(o_tmem, s_tmem + 64 * buffer, tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc_o,
+                   t ? 1u : 0u);
+          tc::commit_w(pv_done + 2 * i + buffer);
+          tc::commit_w(v_empty + s);
+          if (t + 2 < tiles) ok = __all_sync(0xffffffffu, buffer_wait(pv_done, i, n)) && issue_s(t + 2);
         }
         g0 += tiles;
         n0 += tiles;
@@ -379,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 
   const int i = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-  const uint32_t ts = tmem + lanes + S_COL + 64 * i, tp = tmem + lanes + P_COL + 32 * i,
-                 to = tmem + lanes + O_COL + 128 * i;
+  const uint32_t to = tmem + lanes + O_COL + 128 * i;
   const float sl2 = p.scale_log2;
   const int my_token = i * tile_tokens + row / p.group;
   const bool in_tile = row < tile_tokens * p.group;
@@ -401,12 +406,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     const bool warp_live = least != 0x7fffffff;
     float m_used = -INFINITY, l_run = 0.f;
     for (int t = 0; t < tiles; ++t) {
-      const int n = n0 + t;
-      if (!tc::wait(s_full + i, n & 1, abort_flag)) { ok = false; break; }
+      const int n = n0 + t, buffer = n & 1;
+      const uint32_t ts = tmem + lanes + S_COL + 128 * i + 64 * buffer;
+      if (!buffer_wait(s_full, i, n)) { ok = false; break; }
       if (!warp_live) {
-        tc::mbar_arrive(s_empty + i);
-        if (n >= 1 && !tc::wait(pv_done + i, (n - 1) & 1, abort_flag)) { ok = false; break; }
-        tc::mbar_arrive(p_full + i);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full + 2 * i + buffer);
         continue;
       }
       tc::fence_after();
@@ -414,8 +419,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       tc::ld32(ts, r[0]);
       tc::ld32(ts + 32, r[1]);
       tc::wait_ld();
-      tc::fence_before();
-      tc::mbar_arrive(s_empty + i);   // S_i(t + 1) may now be computed into the same columns
       const int key0 = (w.t0 + t) * TK;
       if (key0 + TK > least) {
 #pragma unroll
@@ -458,10 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         acc[(j >> 1) & 3] = __fadd2_rn(acc[(j >> 1) & 3], e);
         packed[j >> 1] = K::pack(e.x, e.y);
       }
-      // P_i(t - 1) V(t - 1) has completed: P_i may be overwritten and O_i holds the products of earlier tiles.
-      if (n >= 1 && !tc::wait(pv_done + i, (n - 1) & 1, abort_flag)) { ok = false; break; }
-      tc::fence_after();
-      if (any_raise && t >= 1) {
+      tc::st32(ts, packed);
+      if (any_raise && t >= 1) {   // O holds the products of the earlier tiles once P(t - 1) V(t - 1) is done
+        if (!buffer_wait(pv_done, i, n - 1)) { ok = false; break; }
+        tc::fence_after();
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -472,14 +475,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           tc::st32(to + c * 32, o);
         }
       }
-      tc::st32(tp, packed);
       tc::wait_st();
       const float2 s01 = __fadd2_rn(acc[0], acc[1]), s23 = __fadd2_rn(acc[2], acc[3]);
       l_run = l_run * alpha + ((s01.x + s01.y) + (s23.x + s23.y));
       tc::fence_before();
-      tc::mbar_arrive(p_full + i);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(p_full + 2 * i + buffer);
     }
-    if (ok) ok = tc::wait(pv_done + i, (n0 + tiles - 1) & 1, abort_flag);
+    if (ok) ok = buffer_wait(pv_done, i, n0 + tiles - 1);
     if (!ok) break;
     tc::fence_after();
     n0 += tiles;
