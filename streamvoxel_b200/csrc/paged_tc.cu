@@ -19,10 +19,12 @@
 // softmax waits for no product but its own tile's. (With one S buffer and P apart the softmax waited 300-450 of the
 // 1,800 cycles of a tile for S: clock stamps.)
 //
-// Warp roles (384 threads): warp 0 loads Q and the K ring, warp 2 the V ring, warps 1 and 3 issue the products of query
-// tiles 0 and 1 (each loop warp-converged, one elected lane issuing), warps 4-7 and 8-11 run their softmax, one row a
-// thread. The exponent base is raised lazily (only when a row's maximum grows by more than 8 in log2 units), a part of
-// the exponentials is evaluated on the FMA pipe; weights are rounded to the cache's type for P V and summed unrounded.
+// Warp roles (448 threads): warp 0 loads Q and the K ring, warp 2 the V ring; warps 1 and 3 issue the scores of query
+// tiles 0 and 1, warps 12 and 13 their products with V (an issuing warp takes a few hundred cycles for a batch of
+// products and its waits, which one warp a tile could not hide); each of these loops is warp-converged, one elected lane
+// issuing. Warps 4-7 and 8-11 run the tiles' softmax, one row a thread. The exponent base is raised lazily (only when a
+// row's maximum grows by more than 8 in log2 units), a part of the exponentials is evaluated on the FMA pipe; weights are
+// rounded to the cache's type for P V and summed unrounded.
 // A query tile without tokens (the second of a short chunk) is skipped by its chain, and a warp without live rows
 // skips the arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
 #include <math.h>
@@ -46,7 +48,7 @@ namespace paged {
 namespace {
 
 constexpr int TQ = 128, TK = kTile;
-constexpr int kThreads = 384;
+constexpr int kThreads = 448;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t S_COL = 0, O_COL = 256;   // + 128 i
 
@@ -85,39 +87,42 @@ __host__ __device__ constexpr uint32_t descriptor(uint32_t format, int m, int n,
          ((uint32_t)(m >> 4) << 24);
 }
 
-// Warp-collective: `Steps` products over 16 of K each, both operands K-major in one 128B-swizzled atom (a step is 32
-// bytes, +2 in descriptor units). acc = 0: the first one starts D afresh.
-template <int Steps>
-__device__ __forceinline__ void mma_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  static_assert(Steps == 2 || Steps == 4, "steps of an atom");
-  if constexpr (Steps == 4) {
-    asm volatile(
-        "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 x, y;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p0;\n\t"
-        "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t"
-        "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t"
-        "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 x, y;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 pt, %3, %3;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p0;\n\t"
-        "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, pt;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc));
-  }
+// One product over 16 of K (operand descriptors %1 and %2 moved on by A and B), and the arrival of a barrier once the
+// products before it are done, both by the elected lane.
+#define SVX_SS_STEP(A, B, ACC)                     \
+  "add.s64 x, %1, " #A ";\n\tadd.s64 y, %2, " #B ";\n\t" \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, " ACC ";\n\t"
+#define SVX_COMMIT(BAR) "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [" BAR "];\n\t"
+
+// Warp-collective: S = Q K^T over D dims, both operands K-major in 128B-swizzled atoms of 64 dims (a step is 32 bytes,
+// +2 in descriptor units; an atom 16 KB of Q and 8 KB of K), then the arrivals on `done` and `release`. One election for
+// the whole batch: an elected block of one instruction costs as much as one of ten.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint64_t q, uint64_t k, uint32_t idesc, uint64_t* done,
+                                             uint64_t* release) {
+#define SVX_SS_BEGIN                                                                     \
+  "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 x, y;\n\telect.sync _|e, 0xffffffff;\n\t" \
+  "setp.ne.b32 p0, %3, %3;\n\tsetp.eq.b32 pt, %3, %3;\n\t"                              \
+  SVX_SS_STEP(0, 0, "p0") SVX_SS_STEP(2, 2, "pt") SVX_SS_STEP(4, 4, "pt") SVX_SS_STEP(6, 6, "pt")
+#define SVX_SS_END SVX_COMMIT("%4") SVX_COMMIT("%5") "}"
+  const uint32_t b0 = smem_addr(done), b1 = smem_addr(release);
+  if constexpr (D == 64)
+    asm volatile(SVX_SS_BEGIN SVX_SS_END ::"r"(d), "l"(q), "l"(k), "r"(idesc), "r"(b0), "r"(b1) : "memory");
+  else if constexpr (D == 96)
+    asm volatile(SVX_SS_BEGIN SVX_SS_STEP(1024, 512, "pt") SVX_SS_STEP(1026, 514, "pt") SVX_SS_END
+                 ::"r"(d), "l"(q), "l"(k), "r"(idesc), "r"(b0), "r"(b1) : "memory");
+  else
+    asm volatile(SVX_SS_BEGIN SVX_SS_STEP(1024, 512, "pt") SVX_SS_STEP(1026, 514, "pt") SVX_SS_STEP(1028, 516, "pt")
+                 SVX_SS_STEP(1030, 518, "pt") SVX_SS_END
+                 ::"r"(d), "l"(q), "l"(k), "r"(idesc), "r"(b0), "r"(b1) : "memory");
+#undef SVX_SS_BEGIN
+#undef SVX_SS_END
 }
 
-// Warp-collective: O += P V over 64 keys: A = P in tensor memory (8 columns a step), B = V MN-major (16 keys x 128 B a
-// step, +128 in descriptor units).
-__device__ __forceinline__ void mma_pv_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Warp-collective: O (+)= P V over 64 keys: A = P in tensor memory (8 columns a step), B = V MN-major (16 keys x 128 B a
+// step, +128 in descriptor units), then the arrivals on `done` and `release`.
+__device__ __forceinline__ void issue_values(uint32_t d, uint32_t p, uint64_t v, uint32_t idesc, uint32_t acc,
+                                             uint64_t* done, uint64_t* release) {
   asm volatile(
       "{\n\t.reg .pred e, p0, pt;\n\t.reg .b64 y;\n\t.reg .b32 x;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
@@ -128,9 +133,12 @@ __device__ __forceinline__ void mma_pv_w(uint32_t d, uint32_t a, uint64_t b, uin
       "add.s32 x, %1, 16;\n\tadd.s64 y, %2, 256;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t"
       "add.s32 x, %1, 24;\n\tadd.s64 y, %2, 384;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, pt;\n\t"
+      SVX_COMMIT("%5") SVX_COMMIT("%6") "}"
+      ::"r"(d), "r"(p), "l"(v), "r"(idesc), "r"(acc), "r"(smem_addr(done)), "r"(smem_addr(release)) : "memory");
 }
+#undef SVX_SS_STEP
+#undef SVX_COMMIT
 
 // max(a, b, c), NaN where any of them is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -319,60 +327,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       }
       if (!ok)   // loads in flight end before the block does
         for (int u = max(0, g - C::stages); u < g; ++u) mbar_wait(full + u % C::stages, (u / C::stages) & 1);
-    } else {   // warp 1: products of query tile 0; warp 3: of query tile 1
+    } else {   // warp 1: scores of query tile 0; warp 3: of query tile 1
       const int i = warp == 1 ? 0 : 1;
-      constexpr uint32_t idesc_s = descriptor(K::format, TQ, TK, false);
-      constexpr uint32_t idesc_o = descriptor(K::format, TQ, D, true);
-      const uint32_t qa = smem_addr(sq + i * C::q_bytes);
-      const uint32_t s_tmem = tmem + S_COL + 128 * i, o_tmem = tmem + O_COL + 128 * i;
-      int g0 = 0, n0 = 0;   // tiles of the ring, and of this chain, before the unit
+      constexpr uint32_t idesc = descriptor(K::format, TQ, TK, false);
+      const uint32_t qa = smem_addr(sq + i * C::q_bytes), d = tmem + S_COL + 128 * i;
+      int g = 0, n = 0;   // tiles of the ring and of this chain
       bool ok = true;
       for (Walk w(p, place); ok && w.more(); w.next(p)) {
-        const int tiles = w.t1 - w.t0;
-        if (i >= live_tiles(p, w.at, tile_tokens)) {   // no rows: hand the tiles back
-          for (int t = 0; ok && t < tiles; ++t) {
-            const int g = g0 + t, s = g % C::stages;
-            ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
-            if (ok && lane == 0) tc::mbar_arrive(k_empty + s);
-            ok = ok && tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
-            if (ok && lane == 0) tc::mbar_arrive(v_empty + s);
-          }
-          if (ok && lane == 0) tc::mbar_arrive(q_empty);
-          g0 += tiles;
-          continue;
-        }
-        if (!tc::wait_w(q_full, w.units & 1, abort_flag)) break;
-        auto issue_s = [&](int t) {   // S(t): its K tile has landed, and its buffer's last P V is done (the caller's wait)
-          const int g = g0 + t, s = g % C::stages;
-          if (!tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag)) return false;
-          tc::fence_after();
-          const uint32_t kb = smem_addr(sk + s * C::k_bytes), buffer = (n0 + t) & 1, d = s_tmem + 64 * buffer;
-          mma_ss_w<4>(d, tc::sw128_desc(qa), tc::sw128_desc(kb), idesc_s, 0u);
-          if constexpr (D > 64)
-            mma_ss_w<(D - 64) / 16>(d, tc::sw128_desc(qa + C::q_atom), tc::sw128_desc(kb + C::k_atom), idesc_s, 1u);
-          tc::commit_w(s_full + 2 * i + buffer);
-          tc::commit_w(k_empty + s);
-          if (t == tiles - 1) tc::commit_w(q_empty);
-          return true;
-        };
-        ok = (n0 == 0 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n0 - 1))) && issue_s(0) && (tiles == 1 || issue_s(1));
-        for (int t = 0; ok && t < tiles; ++t) {   // O += P(t) V(t), which starts O afresh first; then S(t + 2)
-          const int g = g0 + t, n = n0 + t, s = g % C::stages, buffer = n & 1;
-          ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag) &&
-               __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
+        const bool idle = i >= live_tiles(p, w.at, tile_tokens);   // no rows: hand the tiles back
+        if (!idle && !tc::wait_w(q_full, w.units & 1, abort_flag)) { ok = false; break; }
+        for (int t = w.t0; t < w.t1; ++t, ++g) {
+          const int s = g % C::stages;
+          ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
           if (!ok) break;
+          if (idle) {
+            if (lane == 0) tc::mbar_arrive(k_empty + s);
+            continue;
+          }
+          // S(n) goes where P(n - 2) was
+          if (n >= 2 && !__all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2))) { ok = false; break; }
           tc::fence_after();
-          mma_pv_w(o_tmem, s_tmem + 64 * buffer, tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc_o,
-                   t ? 1u : 0u);
-          tc::commit_w(pv_done + 2 * i + buffer);
-          tc::commit_w(v_empty + s);
-          if (t + 2 < tiles) ok = __all_sync(0xffffffffu, buffer_wait(pv_done, i, n)) && issue_s(t + 2);
+          issue_scores<D>(d + 64 * (n & 1), tc::sw128_desc(qa), tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
+                          s_full + 2 * i + (n & 1), k_empty + s);
+          ++n;
         }
-        g0 += tiles;
-        n0 += tiles;
+        if (!ok) break;
+        if (!idle) tc::commit_w(q_empty);
+        else if (lane == 0) tc::mbar_arrive(q_empty);
       }
     }
-    // Teardown: the TMEM owner frees the columns once all 12 warps are past their last TMEM access.
+    // Teardown: the TMEM owner frees the columns once all 14 warps are past their last TMEM access.
     tc::fence_before();
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
@@ -380,6 +364,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       tc::fence_after();
       tc::tmem_dealloc(*tmem_slot, TMEM_COLS);
     }
+    return;
+  }
+
+  if (warp >= 12) {   // warp 12: O of query tile 0; warp 13: of query tile 1
+    const int i = warp - 12;
+    constexpr uint32_t idesc = descriptor(K::format, TQ, D, true);
+    const uint32_t d = tmem + O_COL + 128 * i, a = tmem + S_COL + 128 * i;
+    int g = 0, n = 0;
+    bool ok = true;
+    for (Walk w(p, place); ok && w.more(); w.next(p)) {
+      const bool idle = i >= live_tiles(p, w.at, tile_tokens);
+      for (int t = w.t0; t < w.t1; ++t, ++g) {
+        const int s = g % C::stages;
+        ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
+        if (!ok) break;
+        if (idle) {
+          if (lane == 0) tc::mbar_arrive(v_empty + s);
+          continue;
+        }
+        ok = __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
+        if (!ok) break;
+        tc::fence_after();
+        issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc,
+                     t != w.t0, pv_done + 2 * i + (n & 1), v_empty + s);   // a unit's first product starts O afresh
+        ++n;
+      }
+    }
+    tc::fence_before();
+    __syncwarp();
+    asm volatile("barrier.arrive 1, %0;" ::"n"(kThreads) : "memory");
     return;
   }
 
