@@ -125,13 +125,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
   const uint32_t ring = smem_addr(smem + warp * S::stages * S::stage_bytes);
   grid_launch_dependents();
   grid_dependency_wait();
-  plan<kThreads>(p, cta, gridDim.x, plan_shared);
+  plan<kThreads, false>(p, cta, gridDim.x, plan_shared, nullptr);
   const Place& place = plan_shared.place;
-  const int count = (int)(place.end - place.begin);
-  if (threadIdx.x == 0) {
-    Join* join = reinterpret_cast<Join*>(p.join) + cta;
-    join->valid = 0;
-  }
+  const int count = place.count;
+  if (threadIdx.x == 0) p.join[cta].parts = 0;
   if (count <= 0) return;
 
   // The loading side: a cursor up to stages - 1 tiles ahead, with the next slice's page id already on its way.
@@ -356,16 +353,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
         p.lse[out_row] = sum_r == 0.f ? -INFINITY : (top_r - Half<T>::shift + log2f(sum_r)) * 0.69314718056f;
       }
     }
-    if (threadIdx.x == 0 && segment == 0 && !whole && t == at.tiles) {
-      Join* join = reinterpret_cast<Join*>(p.join) + cta;
-      const int64_t first = place.unit / place.each;
-      join->s = at.s;
-      join->j = at.j;
-      join->h = at.h;
-      join->first = (int)first;
-      join->first_slot = place.unit == first * place.each ? 0 : 1;
-      join->valid = 1;
-    }
+    if (threadIdx.x == 0 && segment == 0 && !whole && t == at.tiles)
+      p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + token0, tokens,
+                         at.h / p.blocks * p.group + g0, part, 0};
     ++segment;
     t = 0;
     at.next(p);
@@ -373,75 +363,78 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
   }
 }
 
-// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, four rows
-// at a time from 4 y on, two warps a row that share its parts.
-template <typename T, int D>
+// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, rows from
+// y * 8 / kWarpsRow on, kWarpsRow warps a row that share its parts. Reads the partial sums once (they are in L2); a chunk's
+// unit has few parts and many rows, a single token's has few rows and up to a part for every CTA.
+template <typename T, int D, int kWarpsRow>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   grid_dependency_wait();
-  const Join join = reinterpret_cast<const Join*>(p.join)[blockIdx.x];
-  if (!join.valid) return;
-  __shared__ float4 s_o[8][32];
-  __shared__ float2 s_ml[8];
-  Cursor at;
-  at.set(p, join.s, join.j, join.h);
-  const int warp = warp_id(), lane = lane_id(), c = blockIdx.x;
-  const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
-  const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
-  const int parts = c - join.first + 1;
-  auto slot = [&](int i) { return 2 * (join.first + i) + (i == 0 ? join.first_slot : 0); };
-  for (int r0 = blockIdx.y * 4; r0 < p.rows; r0 += gridDim.y * 4) {
-    const int r = r0 + warp / 2, in_tile = r % p.tile_rows, token = r / p.tile_rows * p.tile_tokens + in_tile / part;
-    const bool live = in_tile < p.tile_tokens * part && token < tokens;
-    if (!__syncthreads_or(live)) continue;   // also: the last round's shared values have been read
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, total = 0.f;
-    if (live) {
-      for (int i0 = warp & 1; i0 < parts; i0 += 64) {
-        const int i = i0 + 2 * lane;   // this warp's parts: every second one
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (i < parts) ml = p.partial_ml[(int64_t)slot(i) * p.rows + r];
-        float now = ml.x;
+  const Join join = p.join[blockIdx.x];
+  if (!join.parts) return;
+  constexpr int rows = 8 / kWarpsRow;
+  const int warp = warp_id(), lane = lane_id(), share = warp % kWarpsRow;
+  const int r = blockIdx.y * rows + warp / kWarpsRow, in_tile = r % p.tile_rows;
+  const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
+  const bool live = in_tile < p.tile_tokens * join.group && token < join.tokens;
+  auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)) * p.rows + r; };
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, total = 0.f;
+  if (live) {
+    for (int i0 = share; i0 < join.parts; i0 += 32 * kWarpsRow) {
+      const int i = i0 + kWarpsRow * lane;   // this warp's parts
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (i < join.parts) ml = p.partial_ml[slot(i)];
+      float now = ml.x;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-        now = fmaxf(now, top);
-        const float old = top == now ? 1.f : exp2_approx(top - now);
-        const float f = ml.x == now ? 1.f : exp2_approx(ml.x - now);
-        float add = ml.y * f;
+      for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+      now = fmaxf(now, top);
+      const float old = top == now ? 1.f : exp2_approx(top - now);
+      const float f = ml.x == now ? 1.f : exp2_approx(ml.x - now);
+      float add = ml.y * f;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-        total = total * old + add;
-        sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
-        top = now;
-        const int here = min(32, (parts - i0 + 1) / 2);
-#pragma unroll 8
-        for (int x = 0; x < here; ++x) {
-          const float fx = __shfl_sync(0xffffffffu, f, x);
-          if (lane < D / 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p.partial_o + ((int64_t)slot(i0 + 2 * x) * p.rows + r) * D + 4 * lane);
-            sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
-            sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
-          }
+      for (int d = 16; d; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+      total = total * old + add;
+      sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+      top = now;
+      const int here = min(32, (join.parts - i0 + kWarpsRow - 1) / kWarpsRow);
+#pragma unroll 4
+      for (int x = 0; x < here; ++x) {
+        const float fx = __shfl_sync(0xffffffffu, f, x);
+        if (lane < D / 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.partial_o + slot(i0 + kWarpsRow * x) * D + 4 * lane);
+          sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
+          sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
         }
       }
     }
+  }
+  if constexpr (kWarpsRow > 1) {
+    __shared__ float4 s_o[8][32];
+    __shared__ float2 s_ml[8];
     s_o[warp][lane] = sum;
     if (lane == 0) s_ml[warp] = make_float2(top, total);
     __syncthreads();
-    if (!live || (warp & 1)) continue;
-    const float2 other = s_ml[warp + 1];
-    const float4 v = s_o[warp + 1][lane];
-    const float now = fmaxf(top, other.x);
-    const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
-    total = total * f + other.y * g;
-    const float inverse = total == 0.f ? 0.f : 1.f / total;
-    const int64_t out_row = (int64_t)(at.q.row0 + token0 + token) * p.q_heads + at.h / p.blocks * p.group + g0 + in_tile % part;
-    if (lane < D / 4)
-      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
-          make_uint2(Half<T>::pack((sum.x * f + v.x * g) * inverse, (sum.y * f + v.y * g) * inverse),
-                     Half<T>::pack((sum.z * f + v.z * g) * inverse, (sum.w * f + v.w * g) * inverse));
-    if (lane == 0 && p.lse)
-      p.lse[out_row] = total == 0.f ? -INFINITY : (now - Half<T>::shift + log2f(total)) * 0.69314718056f;
+    if (share) return;
+#pragma unroll
+    for (int x = 1; x < kWarpsRow; ++x) {
+      const float2 other = s_ml[warp + x];
+      const float4 v = s_o[warp + x][lane];
+      const float now = fmaxf(top, other.x);
+      const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
+      total = total * f + other.y * g;
+      sum.x = sum.x * f + v.x * g; sum.y = sum.y * f + v.y * g;
+      sum.z = sum.z * f + v.z * g; sum.w = sum.w * f + v.w * g;
+      top = now;
+    }
   }
+  if (!live) return;
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  const int64_t out_row = (int64_t)(join.row + token) * p.q_heads + join.head + in_tile % join.group;
+  if (lane < D / 4)
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
+        make_uint2(Half<T>::pack(sum.x * inverse, sum.y * inverse), Half<T>::pack(sum.z * inverse, sum.w * inverse));
+  if (lane == 0 && p.lse)
+    p.lse[out_row] = total == 0.f ? -INFINITY : (top - Half<T>::shift + log2f(total)) * 0.69314718056f;
 }
 
 int sm_count(int* sms) {
@@ -500,18 +493,20 @@ size_t workspace_bytes(const Division& d, int dim) {
   return (size_t)d.ctas * (sizeof(Join) + 2 * (size_t)d.rows * (dim * sizeof(float) + sizeof(float2)));
 }
 
+template <typename T, int D>
+int launch_all(const Params& p, const Division& d, int dtype, cudaStream_t stream) {
+  const int rc = d.chunk ? chunk_launch(p, dtype, D, d.ctas, stream) : few_rows_launch<T, D>(p, d.ctas, stream);
+  if (rc) return rc;
+  if (d.chunk)
+    return launch_dependent("join_kernel", join_kernel<T, D, 1>, dim3(d.ctas, d.rows / 8), dim3(256), 0, stream, p);
+  return launch_dependent("join_kernel", join_kernel<T, D, 4>, dim3(d.ctas, d.rows / 2), dim3(256), 0, stream, p);
+}
+
 template <typename T>
 int launch_all(const Params& p, const Division& d, int dtype, int dim, cudaStream_t stream) {
-  int rc;
-  if (d.chunk) rc = chunk_launch(p, dtype, dim, d.ctas, stream);
-  else if (dim == 64) rc = few_rows_launch<T, 64>(p, d.ctas, stream);
-  else if (dim == 96) rc = few_rows_launch<T, 96>(p, d.ctas, stream);
-  else rc = few_rows_launch<T, 128>(p, d.ctas, stream);
-  if (rc) return rc;
-  const dim3 grid(d.ctas, d.chunk ? 16 : 4);
-  if (dim == 64) return launch_dependent("join_kernel", join_kernel<T, 64>, grid, dim3(256), 0, stream, p);
-  if (dim == 96) return launch_dependent("join_kernel", join_kernel<T, 96>, grid, dim3(256), 0, stream, p);
-  return launch_dependent("join_kernel", join_kernel<T, 128>, grid, dim3(256), 0, stream, p);
+  if (dim == 64) return launch_all<T, 64>(p, d, dtype, stream);
+  if (dim == 96) return launch_all<T, 96>(p, d, dtype, stream);
+  return launch_all<T, 128>(p, d, dtype, stream);
 }
 
 int check_attention(int tokens, int q_heads, int kv_heads, int dim) {
@@ -571,7 +566,7 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   const size_t slots = 2 * (size_t)d.ctas * d.rows;
   p.partial_o = static_cast<float*>(workspace);
   p.partial_ml = reinterpret_cast<float2*>(p.partial_o + slots * cache->dim);
-  p.join = reinterpret_cast<int32_t*>(p.partial_ml + slots);
+  p.join = reinterpret_cast<paged::Join*>(p.partial_ml + slots);
   p.tokens = tokens;
   p.sequences = cache->sequences;
   p.q_heads = q_heads;

@@ -12,6 +12,8 @@ namespace paged {
 
 constexpr int kTile = 64;   // keys of a step; pages hold 16 * 2^i keys, so a page never straddles a 16-key slice
 
+struct Join;
+
 struct Params {
   const void* q;
   int64_t q_token, q_head;   // strides in elements
@@ -22,7 +24,7 @@ struct Params {
   uint32_t* status;          // [sequences] or null
   float* partial_o;          // [2 ctas][rows][dim]: unnormalised sums of a CTA's first and last unit where it has
   float2* partial_ml;        // [2 ctas][rows]: only a part of it; their exponent bases and sums of exponentials
-  int32_t* join;             // [ctas][8]: the unit that each CTA ends for others (see Join)
+  Join* join;         // [ctas]: the unit that each CTA ends for others
   int tokens, sequences, q_heads, kv_heads, group, page_shift, pages, table_width, causal;
   float scale_log2;
   int unit_tokens;           // tokens of a unit
@@ -33,10 +35,12 @@ struct Params {
   int min_tiles;             // key tiles of a CTA at least
 };
 
-// The work is a line of 64-key tiles: for each sequence, each token tile j, each head h (kv head and part of its group),
-// the tiles of the keys that the token tile can see (one at least, so that rows without keys are written too). CTA c
-// takes an equal run of it, whatever the lengths are; a unit (sequence, j, h) that several CTAs share is joined by a
-// second kernel, always in the same order.
+// The work is a line of 64-key tiles: for each sequence, each head h (kv head and part of its group), each token tile j,
+// the tiles of the keys that the token tile can see (one at least, so that rows without keys are written too). A CTA takes
+// an equal run of the line, whatever the lengths are; a unit (sequence, h, j) that several CTAs share is joined by a
+// second kernel, always in the same order. Calls with several units for each CTA first deal whole units out in waves (CTA
+// c takes units c, c + ctas, ...): the token tiles of one head then run side by side over the same keys, which come from
+// memory once, and only the last units' tiles are divided into runs, whose lengths make every CTA's total equal.
 struct Sequence {
   int row0, n, len;   // first row, new tokens, keys
 };
@@ -96,114 +100,212 @@ __device__ __forceinline__ int64_t tiles_before(const Params& p, const Sequence&
   return sum;
 }
 
-// Where a run of tiles begins.
+// A CTA's share: units cta + k ctas for k < waves, then the run [begin, end) of the line of tiles.
 struct Place {
-  int64_t begin, end;   // run of the CTA on the line of tiles
-  int64_t each;         // tiles of every CTA's run
-  int s, j, h, t;
-  int64_t unit;         // place of its unit's first tile
+  int waves;
+  int s, j, h, t;       // where the run begins
+  int count;            // its tiles
+  int first, first_slot;  // for the join of the unit that the run begins inside of: see Join
 };
 
 struct PlanShared {
-  int64_t warp_sum[32];
+  int64_t warp_tiles[32], warp_units[32];
+  int64_t found[2];     // the run's start on the line, its sequence's start
+  int64_t unit;         // start of the run's first unit
   Place place;
 };
 
-// Fills sh.place for run `c` of `ctas`; all threads of the block call it.
+// Sums over the block of two values; *before: of the threads before this one.
 template <int kThreads>
-__device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShared& sh) {
-  const int heads = p.kv_heads * p.blocks;
-  const int per = (p.sequences + kThreads - 1) / kThreads;
-  const int s0 = min(p.sequences, (int)threadIdx.x * per), s1 = min(p.sequences, s0 + per);
-  int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) {
-    const Sequence q = load_sequence(p, s);
-    mine += tiles_before(p, q, token_tiles(p, q)) * heads;
-  }
-  int64_t sum = mine;
+__device__ __forceinline__ void block_scan(int64_t a, int64_t b, PlanShared& sh, int64_t* before_a, int64_t* before_b,
+                                           int64_t* total_a, int64_t* total_b) {
+  int64_t sa = a, sb = b;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane_id() >= d) sum += o;
-  }
-  if (lane_id() == 31) sh.warp_sum[warp_id()] = sum;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp_id()) before += sh.warp_sum[w];
-    total += sh.warp_sum[w];
-  }
-  before += sum - mine;
-  const int64_t each = max((int64_t)p.min_tiles, (total + ctas - 1) / ctas);
-  const int64_t begin = min(total, each * c), end = min(total, begin + each);
-  if (threadIdx.x == 0) {
-    sh.place.begin = begin;
-    sh.place.end = end;
-    sh.place.each = each;
-  }
-  if (begin < end && begin >= before && begin < before + mine) {
-    int64_t at = before;
-    for (int s = s0; s < s1; ++s) {
-      const Sequence q = load_sequence(p, s);
-      const int tiles = token_tiles(p, q);
-      const int64_t cost = tiles_before(p, q, tiles) * heads;
-      if (begin < at + cost) {
-        int lo = 0, hi = tiles - 1;   // the last token tile that begins at or before the place
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (at + tiles_before(p, q, mid) * heads <= begin) lo = mid; else hi = mid - 1;
-        }
-        at += tiles_before(p, q, lo) * heads;
-        const int each_head = unit_tiles(unit_limit(p, q, lo));
-        const int h = (int)((begin - at) / each_head);
-        sh.place.s = s;
-        sh.place.j = lo;
-        sh.place.h = h;
-        sh.place.unit = at + (int64_t)h * each_head;
-        sh.place.t = (int)(begin - sh.place.unit);
-        break;
-      }
-      at += cost;
+    const int64_t oa = __shfl_up_sync(0xffffffffu, sa, d), ob = __shfl_up_sync(0xffffffffu, sb, d);
+    if (lane_id() >= d) {
+      sa += oa;
+      sb += ob;
     }
   }
   __syncthreads();
+  if (lane_id() == 31) {
+    sh.warp_tiles[warp_id()] = sa;
+    sh.warp_units[warp_id()] = sb;
+  }
+  __syncthreads();
+  *before_a = sa - a;
+  *before_b = sb - b;
+  *total_a = *total_b = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp_id()) {
+      *before_a += sh.warp_tiles[w];
+      *before_b += sh.warp_units[w];
+    }
+    *total_a += sh.warp_tiles[w];
+    *total_b += sh.warp_units[w];
+  }
 }
 
 // A walk over units.
 struct Cursor {
   int s, j, h, limit, tiles;
   Sequence q;
+  __device__ __forceinline__ void see(const Params& p) {
+    limit = unit_limit(p, q, j);
+    tiles = unit_tiles(limit);
+  }
   __device__ __forceinline__ void set(const Params& p, int s_, int j_, int h_) {
     s = s_;
     j = j_;
     h = h_;
     q = load_sequence(p, s);
-    limit = unit_limit(p, q, j);
-    tiles = unit_tiles(limit);
+    see(p);
   }
   __device__ __forceinline__ void next(const Params& p) {
-    if (++h < p.kv_heads * p.blocks) return;
-    h = 0;
     if (++j >= token_tiles(p, q)) {
       j = 0;
-      do {
-        if (++s >= p.sequences) {
-          s = p.sequences - 1;
-          return;
-        }
-        q = load_sequence(p, s);
-      } while (q.n == 0);
+      if (++h >= p.kv_heads * p.blocks) {
+        h = 0;
+        do {
+          if (++s >= p.sequences) {
+            s = p.sequences - 1;
+            return;
+          }
+          q = load_sequence(p, s);
+        } while (q.n == 0);
+      }
     }
-    limit = unit_limit(p, q, j);
-    tiles = unit_tiles(limit);
+    see(p);
+  }
+  // On by `count` units; false past the last one.
+  __device__ __forceinline__ bool skip(const Params& p, int64_t count) {
+    const int heads = p.kv_heads * p.blocks;
+    int per_head = token_tiles(p, q);
+    int64_t at = (int64_t)h * per_head + j + count;
+    while (at >= (int64_t)heads * per_head) {
+      at -= (int64_t)heads * per_head;
+      if (++s >= p.sequences) {
+        s = p.sequences - 1;
+        return false;
+      }
+      q = load_sequence(p, s);
+      per_head = token_tiles(p, q);
+    }
+    h = (int)(at / per_head);
+    j = (int)(at - (int64_t)h * per_head);
+    see(p);
+    return true;
   }
 };
 
-// Left by CTA c for the joining kernel, where its run ends a unit that an earlier CTA began: the unit, the CTA that
-// began it, and whether the unit was that CTA's first (partial slot 2 first) or its last (2 first + 1). The CTAs between
-// hold their parts, like c, in their first slots.
+// Fills sh.place for CTA `c` of `ctas`; all threads of the block call it. kWaves: deal whole units out first where there
+// are enough of them; `scratch` then holds 8 * ctas + 8 bytes of shared memory.
+template <int kThreads, bool kWaves>
+__device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShared& sh, int64_t* scratch) {
+  const int heads = p.kv_heads * p.blocks, tid = threadIdx.x;
+  const int per = (p.sequences + kThreads - 1) / kThreads;
+  const int s0 = min(p.sequences, tid * per), s1 = min(p.sequences, s0 + per);
+  int64_t tiles = 0, units = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Sequence q = load_sequence(p, s);
+    const int n = token_tiles(p, q);
+    tiles += tiles_before(p, q, n) * heads;
+    units += (int64_t)n * heads;
+  }
+  int64_t before, units_before, total, units_total;
+  block_scan<kThreads>(tiles, units, sh, &before, &units_before, &total, &units_total);
+  const int64_t each = max((int64_t)p.min_tiles, (total + ctas - 1) / ctas);
+  int waves = 0;
+  // The last wave and the rest stay for the runs. A step of `ctas` units reads the sequences that it passes, so they are
+  // not to be many.
+  if (kWaves && units_total >= 2 * (int64_t)ctas && units_total >= 16 * (int64_t)p.sequences)
+    waves = (int)min(units_total / ctas - 1, (int64_t)1 << 20);
+  int64_t begin = min(total, each * c), end = min(total, begin + each);
+  if (kWaves && waves) {
+    // Tiles of the units that each CTA takes whole, which are not to be more than its share; then the runs that fill them
+    // up to it.
+    int64_t dealt_tiles = 0;
+    while (true) {
+      dealt_tiles = 0;
+      if (tid < ctas) {
+        Cursor u;
+        u.set(p, 0, 0, 0);
+        bool ok = u.skip(p, tid);
+        for (int k = 0; ok && k < waves; ++k) {
+          dealt_tiles += u.tiles;
+          if (k + 1 < waves) ok = u.skip(p, ctas);
+        }
+      }
+      if (!__syncthreads_or(dealt_tiles > each)) break;
+      waves >>= 1;
+      if (!waves) {
+        dealt_tiles = 0;
+        break;
+      }
+    }
+    const int64_t need = tid < ctas ? each - dealt_tiles : 0;   // waves == 0: equal runs of the whole line
+    int64_t need_before, dealt_before, need_total, dealt_total;
+    block_scan<kThreads>(need, dealt_tiles, sh, &need_before, &dealt_before, &need_total, &dealt_total);
+    if (tid < ctas) scratch[tid] = min(total, dealt_total + need_before);
+    if (tid == 0) scratch[ctas] = total;
+    __syncthreads();
+    begin = scratch[c];
+    end = scratch[c + 1];
+  }
+  if (tid == 0) {
+    sh.place.waves = waves;
+    sh.place.count = (int)(end - begin);
+  }
+  if (begin < end && begin >= before && begin < before + tiles) {
+    int64_t at = before;
+    for (int s = s0; s < s1; ++s) {
+      const Sequence q = load_sequence(p, s);
+      const int n = token_tiles(p, q);
+      const int64_t head = tiles_before(p, q, n);
+      if (begin < at + head * heads) {
+        const int h = (int)((begin - at) / head);
+        at += h * head;
+        int lo = 0, hi = n - 1;   // the last token tile that begins at or before the place
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (at + tiles_before(p, q, mid) <= begin) lo = mid; else hi = mid - 1;
+        }
+        at += tiles_before(p, q, lo);
+        sh.place.s = s;
+        sh.place.j = lo;
+        sh.place.h = h;
+        sh.place.t = (int)(begin - at);
+        // The CTA whose run holds the unit's first tile.
+        int first = (int)(at / each);
+        if (kWaves && waves) {
+          first = 0;
+          int top = c;
+          while (first < top) {
+            const int mid = (first + top + 1) >> 1;
+            if (scratch[mid] <= at) first = mid; else top = mid - 1;
+          }
+        }
+        sh.place.first = first;
+        sh.place.first_slot = at == (kWaves && waves ? scratch[first] : first * each) ? 0 : 1;
+        break;
+      }
+      at += head * heads;
+    }
+  }
+  __syncthreads();
+}
+
+// Left by CTA c for the joining kernel, where its run ends a unit that an earlier CTA began: the unit's rows and heads,
+// the CTA that began it, and whether the unit was that CTA's first of the line (partial slot 2 first) or its last
+// (2 first + 1). The CTAs between hold their parts, like c, in their first slots.
 struct Join {
-  int valid, s, j, h, first, first_slot, pad0, pad1;
+  int parts;               // 0: nothing to join
+  int first, first_slot;
+  int row, tokens;         // its tokens' first row, and their count
+  int head, group;         // its first query head, and their count
+  int pad;
 };
 
 // The form for many rows (paged_tc.cu).

@@ -172,23 +172,47 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // Of every 8 pairs of exponentials, this many go to the FMA pipe.
 constexpr int kPolyPairs = 2;
 
-// A CTA's run, unit by unit: key tiles [t0, t1) of the unit at `at`.
+// A CTA's share, unit by unit: key tiles [t0, t1) of the unit at `at`; `part` counts the units of its run of the line (-1:
+// a unit dealt out whole).
 struct Walk {
   Cursor at;
-  int t0, t1, left, units;
+  int t0, t1, waves, left, units, part;
   __device__ __forceinline__ Walk(const Params& p, const Place& place) {
-    left = (int)(place.end - place.begin);
+    waves = place.waves;
+    left = place.count;
     units = 0;
+    part = -1;
+    t0 = t1 = 0;
+    if (waves) {
+      at.set(p, 0, 0, 0);
+      at.skip(p, blockIdx.x);
+      t1 = at.tiles;
+    } else {
+      start_run(p, place);
+    }
+  }
+  __device__ __forceinline__ void start_run(const Params& p, const Place& place) {
     if (left <= 0) return;
+    part = 0;
     at.set(p, place.s, place.j, place.h);
     t0 = place.t;
     t1 = min(at.tiles, t0 + left);
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  __device__ __forceinline__ void next(const Params& p) {
-    left -= t1 - t0;
+  __device__ __forceinline__ bool more() const { return waves > 0 || left > 0; }
+  __device__ __forceinline__ void next(const Params& p, const Place& place) {
     ++units;
+    if (waves) {
+      if (--waves) {
+        at.skip(p, gridDim.x);
+        t1 = at.tiles;
+      } else {
+        start_run(p, place);
+      }
+      return;
+    }
+    left -= t1 - t0;
     if (left <= 0) return;
+    ++part;
     at.next(p);
     t0 = 0;
     t1 = min(at.tiles, left);
@@ -250,8 +274,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   }
   if (warp == 1) tc::tmem_alloc(tmem_slot, TMEM_COLS);
   grid_dependency_wait();
-  plan<kThreads>(p, cta, gridDim.x, plan_shared);
-  if (threadIdx.x == 0) reinterpret_cast<Join*>(p.join)[cta].valid = 0;
+  plan<kThreads, true>(p, cta, gridDim.x, plan_shared, reinterpret_cast<int64_t*>(smem));   // before the tiles are loaded
+  if (threadIdx.x == 0) p.join[cta].parts = 0;
+  tc::fence_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -295,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         }
         const Cursor at = w.at;
         const int t0 = w.t0, t1 = w.t1;
-        w.next(p);
+        w.next(p, place);
         for (int t = t0; t < t1; ++t, ++g) {
           const int s = g % C::stages;
           if (g >= C::stages && !tc::wait_w(empty + s, (g / C::stages - 1) & 1, abort_flag)) { ok = false; break; }
@@ -333,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       const uint32_t qa = smem_addr(sq + i * C::q_bytes), d = tmem + S_COL + 128 * i;
       int g = 0, n = 0;   // tiles of the ring and of this chain
       bool ok = true;
-      for (Walk w(p, place); ok && w.more(); w.next(p)) {
+      for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
         const bool idle = i >= live_tiles(p, w.at, tile_tokens);   // no rows: hand the tiles back
         if (!idle && !tc::wait_w(q_full, w.units & 1, abort_flag)) { ok = false; break; }
         for (int t = w.t0; t < w.t1; ++t, ++g) {
@@ -373,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     const uint32_t d = tmem + O_COL + 128 * i, a = tmem + S_COL + 128 * i;
     int g = 0, n = 0;
     bool ok = true;
-    for (Walk w(p, place); ok && w.more(); w.next(p)) {
+    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
       const bool idle = i >= live_tiles(p, w.at, tile_tokens);
       for (int t = w.t0; t < w.t1; ++t, ++g) {
         const int s = g % C::stages;
@@ -403,10 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const float sl2 = p.scale_log2;
   const int my_token = i * tile_tokens + row / p.group;
   const bool in_tile = row < tile_tokens * p.group;
-  int n0 = 0, unit = 0;
+  int n0 = 0;
   bool ok = true;
   Walk w(p, place);
-  for (; ok && w.more(); w.next(p), ++unit) {
+  for (; ok && w.more(); w.next(p, place)) {
     const Cursor& at = w.at;
     if (p.status && threadIdx.x == 128) {
       if (__ldg(p.lengths + at.s) != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
@@ -501,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     tc::fence_after();
     n0 += tiles;
     const bool whole = w.t0 == 0 && w.t1 == at.tiles;
-    const int64_t slot = (int64_t)(2 * cta + (unit ? 1 : 0)) * p.rows + i * TQ + row;
+    const int64_t slot = (int64_t)(2 * cta + (w.part > 0 ? 1 : 0)) * p.rows + i * TQ + row;
     const int64_t out_row = (int64_t)(at.q.row0 + token) * p.q_heads + at.h * p.group + row % p.group;
     // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
     // makes the row NaN, as inf - inf does.
@@ -535,16 +560,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       if (live && whole && p.lse)
         p.lse[out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
     }
-    if (threadIdx.x == 128 && unit == 0 && !whole && w.t1 == at.tiles) {
-      Join* join = reinterpret_cast<Join*>(p.join) + cta;
-      const int64_t first = place.unit / place.each;
-      join->s = at.s;
-      join->j = at.j;
-      join->h = at.h;
-      join->first = (int)first;
-      join->first_slot = place.unit == first * place.each ? 0 : 1;
-      join->valid = 1;
-    }
+    if (threadIdx.x == 128 && w.part == 0 && !whole && w.t1 == at.tiles)
+      p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + at.j * p.unit_tokens,
+                         min(p.unit_tokens, at.q.n - at.j * p.unit_tokens), at.h * p.group, p.group, 0};
     // O_i has been read; the next unit's first P V, which overwrites it, is issued only after this warpgroup's next
     // p_full arrival.
     tc::fence_before();

@@ -388,6 +388,19 @@ def test_attention_many_sequences(ops):
     _check(ops, g, q, k_pages, v_pages, table, lengths, _offsets(news), True, max_query=90)
 
 
+@pytest.mark.parametrize('news,keys', [([600, 500, 700, 20, 650], [900, 500, 700, 3000, 651]),
+                                       ([700, 1, 1, 700, 700, 700], [700, 9000, 5, 800, 2000, 710]),
+                                       ([1400, 1100], [1400, 7000])])
+def test_attention_many_units(ops, news, keys):
+    """Enough token tiles to deal whole ones out to the CTAs before the rest is divided; lengths that make the dealt ones
+    unequal."""
+    rng, g = np.random.default_rng(11), torch.Generator().manual_seed(11)
+    k_pages, v_pages, table, lengths = _cache(rng, keys, 8, 64, 64, torch.bfloat16)
+    _fill((k_pages, v_pages), table, lengths, g)
+    q = torch.randn((sum(news), 32, 64), generator=g).bfloat16().cuda()
+    _check(ops, g, q, k_pages, v_pages, table, lengths, _offsets(news), True, max_query=max(news))
+
+
 def test_attention_shared_pages(ops):
     """Sequences whose tables begin with the same pages (a shared prefix)."""
     rng, g = np.random.default_rng(9), torch.Generator().manual_seed(9)
