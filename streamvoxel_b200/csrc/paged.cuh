@@ -109,9 +109,7 @@ struct Place {
 };
 
 struct PlanShared {
-  int64_t warp_tiles[32], warp_units[32];
-  int64_t found[2];     // the run's start on the line, its sequence's start
-  int64_t unit;         // start of the run's first unit
+  int64_t warp_tiles[16], warp_units[16];   // of at most 512 threads
   Place place;
 };
 
