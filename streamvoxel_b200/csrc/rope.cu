@@ -6,24 +6,27 @@
 // flipped. Interleaved pairs are (2j, 2j + 1), half pairs (j, j + rot / 2); with several position axes the pairs are
 // split evenly among them, axis-major (the axial rotation of the GEMM epilogue).
 //
-// Both operators are one pass over their rows and bound by memory once the rows outgrow L2. A CTA takes a few tokens:
-// it first computes the tokens' cosines and sines into shared memory, once for all heads, then moves 16-byte vectors.
-// The angle is formed in float64 and reduced to a fraction of a turn there (positions of a million lose 2e-2 of a
-// radian in 32 bits), the rest is fp32; a value is rounded to its own type once.
+// Both operators are one pass over their rows and bound by memory once the rows outgrow L2, if they spend few instructions
+// and keep many loads in flight. A warp takes a token (or, of few tokens, a share of one): it sets off its first rows' loads
+// of 16 bytes a lane, then looks up the token's place in the cache and computes its cosines and sines, once for all heads,
+// which hides that chain of small loads behind the rows; no step waits for another warp. The angle is formed in float64
+// and reduced to an eighth of a turn there (positions of a million lose 2e-2 of a radian in 32 bits), the rest is fp32; a
+// value is rounded to its own type once.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.cuh"
 
 namespace svx {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTile = kThreads / 32;   // tokens of a CTA: a warp looks up each token's sequence
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxPairs = 256;
 
-// One source of rows: [tokens][heads][dim] with strides in elements; the destination likewise, or the cache's pages.
+// Rows to move: [tokens][heads][dim] with strides in elements.
 struct Rows {
   const void* src;
-  void* dst;
+  void* dst;             // q: strided like src; k, v: the pool
   int64_t src_token, src_head, dst_token, dst_head;
   int heads;
 };
@@ -34,8 +37,11 @@ struct MoveParams {
   const void* positions;      // null: the token's position in the cache
   int position_type, axes, pairs, layout, inverse;
   float scale;
-  int tokens, dim, tile;
-  // cache (sequences == 0: none)
+  int tokens, dim;
+  int parts;                  // warps of a token
+  int items;                  // of a head, see move_rows_kernel
+  int step_heads, step_items; // 32 * parts items on, in heads and items
+  // cache
   const int32_t *table, *lengths, *offsets;
   uint32_t* status;
   int sequences, table_width, pages, page_shift;
@@ -49,142 +55,261 @@ template <> __device__ __forceinline__ float from_f32<float>(float f) { return f
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float f) { return __float2bfloat16_rn(f); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float f) { return __float2half_rn(f); }
 
-template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+// N values: one of them, or 16 bytes as words (two 16-bit values or one fp32 value a word).
+template <typename T, int N> struct Pack { uint4 w; };
+template <typename T> struct Pack<T, 1> { T v; };
 
-// N = 1 is the form for any dim, stride and alignment; N = 16 bytes' worth needs all of them in whole vectors.
-template <typename T, int N>
+__device__ __forceinline__ float2 unpack(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack(__nv_bfloat16, float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack(__half, float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+
+// (f, g) turned by the angle with cosine c and sine s.
+__device__ __forceinline__ float2 turned(float f, float g, float c, float s) {
+  return make_float2(f * c - g * s, f * s + g * c);
+}
+
+// Whole pairs within a vector; cs: their (cos, sin).
+template <typename T>
+__device__ __forceinline__ void turn_inside(uint4& a, const float2* cs) {
+  const float4 x = reinterpret_cast<const float4*>(cs)[0];
+  if constexpr (sizeof(T) == 4) {
+    const float2 u = turned(__uint_as_float(a.x), __uint_as_float(a.y), x.x, x.y);
+    const float2 v = turned(__uint_as_float(a.z), __uint_as_float(a.w), x.z, x.w);
+    a = make_uint4(__float_as_uint(u.x), __float_as_uint(u.y), __float_as_uint(v.x), __float_as_uint(v.y));
+  } else {
+    const float4 y = reinterpret_cast<const float4*>(cs)[1];
+    auto word = [](uint32_t w, float c, float s) {
+      const float2 f = unpack(T(), w), u = turned(f.x, f.y, c, s);
+      return pack(T(), u.x, u.y);
+    };
+    a = make_uint4(word(a.x, x.x, x.y), word(a.y, x.z, x.w), word(a.z, y.x, y.y), word(a.w, y.z, y.w));
+  }
+}
+
+// Pairs across two vectors.
+template <typename T>
+__device__ __forceinline__ void turn_across(uint4& a, uint4& b, const float2* cs) {
+  if constexpr (sizeof(T) == 4) {
+    auto word = [](uint32_t& f, uint32_t& g, float2 t) {
+      const float2 u = turned(__uint_as_float(f), __uint_as_float(g), t.x, t.y);
+      f = __float_as_uint(u.x);
+      g = __float_as_uint(u.y);
+    };
+    word(a.x, b.x, cs[0]);
+    word(a.y, b.y, cs[1]);
+    word(a.z, b.z, cs[2]);
+    word(a.w, b.w, cs[3]);
+  } else {
+    auto word = [](uint32_t& f, uint32_t& g, float4 t) {
+      const float2 x = unpack(T(), f), y = unpack(T(), g);
+      const float2 u = turned(x.x, y.x, t.x, t.y), v = turned(x.y, y.y, t.z, t.w);
+      f = pack(T(), u.x, v.x);
+      g = pack(T(), u.y, v.y);
+    };
+    const float4* at = reinterpret_cast<const float4*>(cs);
+    word(a.x, b.x, at[0]);
+    word(a.y, b.y, at[1]);
+    word(a.z, b.z, at[2]);
+    word(a.w, b.w, at[3]);
+  }
+}
+
+// (cos, sin) of 2 pi turns. The turns are reduced to [-1/8, 1/8] in float64, then sine and cosine are their Taylor series up
+// to x^9 and x^10 (|x| <= pi / 4: the next terms are under 2e-9), and the quarter turns swap and negate them.
+__device__ __forceinline__ float2 cos_sin_turns(double turns) {
+  // Adding 1.5 * 2^52 rounds to a whole number, which then stands in the low bits (|turns| < 2^49); a rounding and a
+  // conversion to integers would take the slow conversion pipe.
+  const double sum = fma(4.0, turns, 6755399441055744.0), quarters = sum - 6755399441055744.0;
+  const float x = (float)(fma(-0.25, quarters, turns) * 6.283185307179586477);
+  const int k = __double2loint(sum) & 3;
+  const float z = x * x;
+  float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
+  s = fmaf(z, s, 8.3333333e-3f);
+  s = fmaf(z, s, -1.6666667e-1f);
+  s = fmaf(z * x, s, x);
+  float c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+  c = fmaf(z, c, -1.3888889e-3f);
+  c = fmaf(z, c, 4.1666667e-2f);
+  c = fmaf(z, c, -0.5f);
+  c = fmaf(z, c, 1.f);
+  const float cs = k & 1 ? s : c, sn = k & 1 ? c : s;
+  return make_float2(k == 1 || k == 2 ? -cs : cs, k >= 2 ? -sn : sn);
+}
+
+// An item of a head is N values, or N and their N partners (kPaired): vectors of the interleaved layout hold whole pairs,
+// those of the half layout and single values (N = 1, the form for any dim, stride and alignment) come with a partner.
+// Items past the turned values are N values without a partner.
+template <typename T, int N, bool kPaired>
+struct Items {
+  using P = Pack<T, N>;
+  const MoveParams& p;
+  int turning, rot, partner, first_head, first_item;
+
+  __device__ __forceinline__ Items(const MoveParams& p_, int start) : p(p_) {
+    rot = p.inv_freq ? 2 * p.pairs : 0;
+    turning = kPaired ? rot / (2 * N) : rot / N;
+    partner = p.layout == SVX_ROPE_HALF ? p.pairs : 1;
+    first_head = start / p.items;
+    first_item = start - first_head * p.items;
+  }
+  __device__ __forceinline__ int value(int item) const {   // the first value of an item
+    if (!kPaired) return item * N;
+    if (item >= turning) return rot + (item - turning) * N;
+    return N == 1 && p.layout != SVX_ROPE_HALF ? 2 * item : item * N;
+  }
+  __device__ __forceinline__ void advance(int* head, int* item) const {
+    *head += p.step_heads;
+    *item += p.step_items;
+    if (*item >= p.items) {
+      *item -= p.items;
+      ++*head;
+    }
+  }
+  __device__ __forceinline__ void load(const T* src, int item, P* a, P* b) const {
+    *a = *reinterpret_cast<const P*>(src);
+    if (kPaired && item < turning) *b = *reinterpret_cast<const P*>(src + partner);
+  }
+  __device__ __forceinline__ void turn(const float2* angles, int item, P* a, P* b) const {
+    if (item >= turning) return;
+    if constexpr (N == 1) {
+      const float2 cs = angles[item], u = turned(to_f32(a->v), to_f32(b->v), cs.x, cs.y);
+      a->v = from_f32<T>(u.x);
+      b->v = from_f32<T>(u.y);
+    } else if constexpr (kPaired) {
+      turn_across<T>(a->w, b->w, angles + item * N);
+    } else {
+      turn_inside<T>(a->w, angles + item * (N / 2));
+    }
+  }
+  __device__ __forceinline__ void store(T* dst, int item, const P& a, const P& b) const {
+    *reinterpret_cast<P*>(dst) = a;
+    if (kPaired && item < turning) *reinterpret_cast<P*>(dst + partner) = b;
+  }
+};
+
+template <typename T, int N, bool kPaired, bool kPaged>
 __global__ void __launch_bounds__(kThreads) move_rows_kernel(const MoveParams p) {
-  __shared__ float2 s_turn[kMaxTile * kMaxPairs];   // (cos, sin) * scale, indexed [token][pair]
-  __shared__ int64_t s_row[kMaxTile];      // row of the token's key in head 0 of its page, -1: not stored
-  __shared__ int s_at[kMaxTile];           // position in the cache
-  __shared__ int s_live[kMaxTile];         // 0: the token belongs to no sequence
+  // Items of a lane in flight, of q alone and of k and v together.
+  constexpr int kQ = kPaged ? (kPaired ? 1 : 2) : (kPaired ? 3 : 6), kKv = kPaired ? 2 : 3;
+  __shared__ __align__(16) float2 s_turn[kWarps][kMaxPairs];   // (cos, sin) * scale
   using P = Pack<T, N>;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int token0 = blockIdx.x * p.tile, tile = min(p.tile, p.tokens - token0);
-  if (p.sequences) {
-    const int w = warp_id();
-    if (w < tile) {
-      const int t = token0 + w;
-      // The token's sequence is the count of sequence ends at or before it; every lane's loads are independent.
-      int count = 0;
-      for (int i = lane_id(); i < p.sequences; i += 32) count += __ldg(p.offsets + i + 1) <= t;
-      const int s = __reduce_add_sync(0xffffffffu, count);
-      if (lane_id() == 0) {
-        int at = 0;
-        int64_t row = -1;
-        bool live = false;
-        if (s < p.sequences) {
-          const int first = p.offsets[s], end = p.offsets[s + 1];
-          live = t >= first;
-          if (live) {
-            const int64_t place = (int64_t)p.lengths[s] - end + t;
-            bool ok = place >= 0 && place < ((int64_t)p.table_width << p.page_shift);
-            at = (int)max((int64_t)-(1 << 30), min(place, (int64_t)1 << 30));
-            if (ok && p.k.heads) {
-              const int page = p.table[(int64_t)s * p.table_width + (place >> p.page_shift)];
-              ok = page >= 0 && page < p.pages;
-              if (ok) row = ((int64_t)page * p.k.heads << p.page_shift) + (place & ((1 << p.page_shift) - 1));
-            }
-            if (!ok && p.status) atomicOr(p.status + s, SVX_STATUS_BAD_PAGE);
-          }
-        }
-        s_at[w] = at;
-        s_row[w] = row;
-        s_live[w] = live;
-      }
+  const int unit = blockIdx.x * kWarps + warp_id(), lane = lane_id();
+  const int t = unit / p.parts, part = unit - t * p.parts;
+  if (t >= p.tokens) return;
+  const Items<T, N, kPaired> items(p, lane + 32 * part);
+  const T* q_src = static_cast<const T*>(p.q.src) + (int64_t)t * p.q.src_token;
+  T* q_dst = static_cast<T*>(p.q.dst) + (int64_t)t * p.q.dst_token;
+  const T* k_src = static_cast<const T*>(p.k.src) + (int64_t)t * p.k.src_token;
+  const T* v_src = static_cast<const T*>(p.v.src) + (int64_t)t * p.v.src_token;
+
+  P qa[kQ], qb[kPaired ? kQ : 1], ka[kKv], kb[kPaired ? kKv : 1], va[kKv], vb[kPaired ? kKv : 1];
+  auto load_q = [&](int head, int item) {
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      if (head < p.q.heads)
+        items.load(q_src + (int64_t)head * p.q.src_head + items.value(item), item, qa + u, qb + (kPaired ? u : 0));
+      items.advance(&head, &item);
     }
-    __syncthreads();
+  };
+  auto load_kv = [&](int head, int item) {
+#pragma unroll
+    for (int u = 0; u < kKv; ++u) {
+      if (head < p.k.heads) {
+        const int value = items.value(item);
+        items.load(k_src + (int64_t)head * p.k.src_head + value, item, ka + u, kb + (kPaired ? u : 0));
+        items.load(v_src + (int64_t)head * p.v.src_head + value, item, va + u, vb + (kPaired ? u : 0));
+      }
+      items.advance(&head, &item);
+    }
+  };
+  if (kPaged) load_kv(items.first_head, items.first_item);
+  load_q(items.first_head, items.first_item);
+
+  int place = 0;       // the token's position in the cache
+  int64_t row = -1;    // the row of its key in head 0 of its page, -1: not stored
+  if (kPaged) {
+    // The token's sequence is the count of sequence ends at or before it; every lane's loads are independent.
+    int count = 0;
+    for (int i = lane; i < p.sequences; i += 32) count += __ldg(p.offsets + i + 1) <= t;
+    const int s = __reduce_add_sync(0xffffffffu, count);
+    if (s >= p.sequences) return;
+    const int begin = __ldg(p.offsets + s), end = __ldg(p.offsets + s + 1), length = __ldg(p.lengths + s);
+    if (t < begin) return;
+    const int64_t at = (int64_t)length - end + t;
+    bool ok = at >= 0 && at < ((int64_t)p.table_width << p.page_shift);
+    place = (int)max((int64_t)-(1 << 30), min(at, (int64_t)1 << 30));
+    if (ok) {
+      const int page = __ldg(p.table + (int64_t)s * p.table_width + (at >> p.page_shift));
+      ok = page >= 0 && page < p.pages;
+      if (ok) row = ((int64_t)page * p.k.heads << p.page_shift) + (at & ((1 << p.page_shift) - 1));
+    }
+    if (!ok && p.status && lane == 0 && part == 0) atomicOr(p.status + s, SVX_STATUS_BAD_PAGE);
   }
+  float2* angles = s_turn[warp_id()];
   if (p.inv_freq) {
     const int per_axis = p.pairs / p.axes;
-    for (int i = threadIdx.x; i < tile * p.pairs; i += kThreads) {
-      const int w = i / p.pairs, j = i - w * p.pairs;
-      double position;
-      if (!p.positions) {
-        position = s_at[w];
-      } else {
-        const int64_t e = (int64_t)(token0 + w) * p.axes + j / per_axis;
+    for (int j = lane; j < p.pairs; j += 32) {
+      double position = place;
+      if (p.positions) {
+        int64_t e = (int64_t)t * p.axes;
+        for (int a = per_axis; a <= j; a += per_axis) ++e;   // the pair's axis
         position = p.position_type == SVX_I64   ? (double)static_cast<const int64_t*>(p.positions)[e]
                    : p.position_type == SVX_I32 ? (double)static_cast<const int32_t*>(p.positions)[e]
                                                 : (double)static_cast<const float*>(p.positions)[e];
       }
-      double turns = position * p.inv_freq[j] * 0.15915494309189533577;   // 1 / (2 pi)
-      turns -= rint(turns);
-      // The fraction of a turn as the nearest float and a first-order correction for what that drops.
-      const float near = (float)turns, rest = (float)(turns - (double)near) * 6.2831853f;
-      float sn, cs;
-      sincospif(2.f * near, &sn, &cs);
-      const float c = fmaf(-rest, sn, cs), s = fmaf(rest, cs, sn);
-      s_turn[i] = make_float2(c * p.scale, (p.inverse ? -s : s) * p.scale);
+      const float2 cs = cos_sin_turns(position * p.inv_freq[j] * 0.15915494309189533577);   // 1 / (2 pi)
+      angles[j] = make_float2(cs.x * p.scale, (p.inverse ? -cs.y : cs.y) * p.scale);
     }
-    __syncthreads();
+    __syncwarp();
   }
-  // Items of a token: for each head its vectors; of the half layout the first rot / 2 values' items carry their
-  // partners with them. `plain` items are copied.
-  const bool half = p.layout == SVX_ROPE_HALF && p.inv_freq;
-  const int turning = p.inv_freq ? (N == 1 || half ? p.pairs / (N == 1 ? 1 : N) : 2 * p.pairs / N) : 0;
-  const int plain = (p.dim - (p.inv_freq ? 2 * p.pairs : 0)) / N;
-  const int per_turned = turning + plain, per_copied = p.dim / N;
-  const int n_turned = (p.q.heads + p.k.heads) * per_turned, per_token = n_turned + p.v.heads * per_copied;
-  for (int i = threadIdx.x; i < tile * per_token; i += kThreads) {
-    const int w = i / per_token;
-    int r = i - w * per_token;
-    const bool copied = r >= n_turned;
-    int head, item;
-    if (copied) {
-      r -= n_turned;
-      head = r / per_copied;
-      item = r - head * per_copied;
-    } else {
-      head = r / per_turned;
-      item = r - head * per_turned;
-    }
-    if (p.sequences && !s_live[w]) continue;
-    const int64_t t = token0 + w;
-    const bool is_k = !copied && head >= p.q.heads;
-    const T* src;
-    T* dst;
-    if (copied || is_k) {
-      if (is_k) head -= p.q.heads;
-      if (s_row[w] < 0) continue;
-      const int64_t row = s_row[w] + ((int64_t)head << p.page_shift);
-      src = static_cast<const T*>(copied ? p.v.src : p.k.src) + t * (copied ? p.v.src_token : p.k.src_token) +
-            head * (copied ? p.v.src_head : p.k.src_head);
-      dst = static_cast<T*>(copied ? p.v.dst : p.k.dst) + row * p.dim;
-    } else {
-      src = static_cast<const T*>(p.q.src) + t * p.q.src_token + head * p.q.src_head;
-      dst = static_cast<T*>(p.q.dst) + t * p.q.dst_token + head * p.q.dst_head;
-    }
-    const float2* turn = s_turn + w * p.pairs;
-    if (copied || item >= turning) {
-      const int e = copied ? item * N : p.dim - (per_turned - item) * N;
-      *reinterpret_cast<P*>(dst + e) = *reinterpret_cast<const P*>(src + e);
-    } else if (N == 1 || half) {
-      const int a = half ? item * N : 2 * item, b = half ? a + p.pairs : a + 1;
-      const P x = *reinterpret_cast<const P*>(src + a), y = *reinterpret_cast<const P*>(src + b);
-      P u, v;
+
+  if (kPaged && row >= 0) {
+    T* k_dst = static_cast<T*>(p.k.dst) + row * p.dim;
+    T* v_dst = static_cast<T*>(p.v.dst) + row * p.dim;
+    const int64_t head_stride = (int64_t)p.dim << p.page_shift;
+    int head = items.first_head, item = items.first_item;
+    while (head < p.k.heads) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float2 cs = turn[item * N + e];
-        const float f = to_f32(x.v[e]), g = to_f32(y.v[e]);
-        u.v[e] = from_f32<T>(f * cs.x - g * cs.y);
-        v.v[e] = from_f32<T>(f * cs.y + g * cs.x);
+      for (int u = 0; u < kKv; ++u) {
+        if (head < p.k.heads) {
+          const int64_t offset = head * head_stride + items.value(item);
+          constexpr int second = kPaired ? 1 : 0;
+          items.turn(angles, item, ka + u, kb + u * second);
+          items.store(k_dst + offset, item, ka[u], kb[u * second]);
+          items.store(v_dst + offset, item, va[u], vb[u * second]);
+        }
+        items.advance(&head, &item);
       }
-      *reinterpret_cast<P*>(dst + a) = u;
-      *reinterpret_cast<P*>(dst + b) = v;
-    } else {
-      const P x = *reinterpret_cast<const P*>(src + item * N);
-      P u;
-#pragma unroll
-      for (int e = 0; e + 1 < N; e += 2) {
-        const float2 cs = turn[(item * N + e) / 2];
-        const float f = to_f32(x.v[e]), g = to_f32(x.v[e + 1]);
-        u.v[e] = from_f32<T>(f * cs.x - g * cs.y);
-        u.v[e + 1] = from_f32<T>(f * cs.y + g * cs.x);
-      }
-      *reinterpret_cast<P*>(dst + item * N) = u;
+      load_kv(head, item);
     }
+  }
+  int head = items.first_head, item = items.first_item;
+  while (head < p.q.heads) {
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      if (head < p.q.heads) {
+        constexpr int second = kPaired ? 1 : 0;
+        items.turn(angles, item, qa + u, qb + u * second);
+        items.store(q_dst + (int64_t)head * p.q.dst_head + items.value(item), item, qa[u], qb[u * second]);
+      }
+      items.advance(&head, &item);
+    }
+    load_q(head, item);
   }
 }
 
@@ -196,27 +321,24 @@ bool whole(const Rows& r, int n, size_t size) {
          r.dst_head % n == 0;
 }
 
-template <typename T>
+template <typename T, bool kPaged>
 int launch_move(MoveParams p, cudaStream_t stream) {
   constexpr int n = 16 / sizeof(T);
-  const bool half = p.layout == SVX_ROPE_HALF;
+  const bool half = p.layout == SVX_ROPE_HALF && p.inv_freq;
   const bool wide = p.dim % n == 0 && (!p.inv_freq || (half ? p.pairs % n == 0 : 2 * p.pairs % n == 0)) &&
                     whole(p.q, n, sizeof(T)) && whole(p.k, n, sizeof(T)) && whole(p.v, n, sizeof(T));
-  // Tokens of a CTA: about four vectors a thread, but no fewer CTAs than two for each SM.
-  const int64_t vectors = (int64_t)(p.q.heads + p.k.heads + p.v.heads) * p.dim / (wide ? n : 2);
-  int tile = (int)(4 * kThreads / (vectors > 0 ? vectors : 1));
-  tile = tile < 1 ? 1 : tile > kMaxTile ? kMaxTile : tile;
-  while (tile > 1 && p.tokens / tile < 296) tile >>= 1;
-  p.tile = tile;
-  const dim3 grid((p.tokens + tile - 1) / tile);
-  if (wide) return launch_dependent("move_rows_kernel", move_rows_kernel<T, n>, grid, dim3(kThreads), 0, stream, p);
-  return launch_dependent("move_rows_kernel", move_rows_kernel<T, 1>, grid, dim3(kThreads), 0, stream, p);
-}
-
-int launch_move(const MoveParams& p, int dtype, cudaStream_t stream) {
-  if (dtype == SVX_BF16) return launch_move<__nv_bfloat16>(p, stream);
-  if (dtype == SVX_F16) return launch_move<__half>(p, stream);
-  return launch_move<float>(p, stream);
+  const int width = wide ? n : 1, rot = p.inv_freq ? 2 * p.pairs : 0;
+  p.items = (!wide || half ? rot / (2 * width) : rot / width) + (p.dim - rot) / width;
+  // Warps of a token: one, or as many as there is work for while they are fewer than 16 a SM.
+  const int64_t items = (int64_t)std::max(p.q.heads, p.k.heads) * p.items;
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>((items + 31) / 32, 2368 / p.tokens));
+  p.step_heads = 32 * p.parts / p.items;
+  p.step_items = 32 * p.parts % p.items;
+  const int64_t units = (int64_t)p.tokens * p.parts;
+  const dim3 grid((unsigned)((units + kWarps - 1) / kWarps));
+  auto kernel = !wide ? move_rows_kernel<T, 1, true, kPaged>
+                : half ? move_rows_kernel<T, n, true, kPaged> : move_rows_kernel<T, n, false, kPaged>;
+  return launch_dependent("move_rows_kernel", kernel, grid, dim3(kThreads), 0, stream, p);
 }
 
 int take_rotary(const svx_rotary* r, int dim, MoveParams* p) {
@@ -259,7 +381,9 @@ extern "C" int svx_rope(const void* x, int dtype, int64_t x_token_stride, int64_
   p.inverse = inverse != 0;
   p.tokens = tokens;
   p.dim = dim;
-  return launch_move(p, dtype, as_stream(stream));
+  if (dtype == SVX_BF16) return launch_move<__nv_bfloat16, false>(p, as_stream(stream));
+  if (dtype == SVX_F16) return launch_move<__half, false>(p, as_stream(stream));
+  return launch_move<float, false>(p, as_stream(stream));
 }
 
 extern "C" int svx_paged_append(const svx_paged_cache* cache, const void* k, int64_t k_token_stride,
@@ -288,5 +412,6 @@ extern "C" int svx_paged_append(const svx_paged_cache* cache, const void* k, int
   p.table_width = cache->table_width;
   p.pages = cache->pages;
   p.page_shift = shift;
-  return launch_move(p, cache->dtype, as_stream(stream));
+  if (cache->dtype == SVX_BF16) return launch_move<__nv_bfloat16, true>(p, as_stream(stream));
+  return launch_move<__half, true>(p, as_stream(stream));
 }
