@@ -47,7 +47,6 @@ namespace paged {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 16;
-constexpr int kCtasPerSm = 2;
 
 template <typename T> struct Half;   // the two 16-bit types
 template <> struct Half<__nv_bfloat16> {
@@ -107,20 +106,21 @@ template <int D> struct Shape {
   static constexpr int chunks = D / 8;                  // 16-byte pieces of a row
   static constexpr int row_bytes = (chunks + 1) * 16;   // odd in 16-byte units: ldmatrix rows fall into distinct banks
   static constexpr int stage_bytes = 2 * 16 * row_bytes;
-  // Enough keys in flight for the memory's latency (about 64 KB a SM) with two CTAs a SM: measured below.
-  static constexpr int stages = D == 64 ? 6 : D == 96 ? 4 : 3;
-  static constexpr int merge_stride = 40;               // floats of a merged row's 32 values, padded
-  static constexpr size_t smem =
-      (size_t)kWarps * stages * stage_bytes + (size_t)kWarps * kRows * merge_stride * 4;
+  // CTAs of a SM and stages of a warp's ring: what keeps the most keys in flight within the registers (128, 168 and 220 a
+  // thread) and shared memory.
+  static constexpr int ctas_per_sm = D == 64 ? 4 : D == 96 ? 3 : 2;
+  static constexpr int stages = D == 128 ? 3 : 2;
+  static constexpr int merge_stride = D + 8;            // floats of a merged row: conflict-free for the fragments' layout
+  static_assert(kRows * merge_stride * 4 <= stage_bytes, "a warp's part of a unit takes the place of a stage");
+  static constexpr size_t smem = (size_t)kWarps * stages * stage_bytes;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kernel(const Params p) {
   using S = Shape<D>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ PlanShared plan_shared;
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-  float* merge = reinterpret_cast<float*>(smem + kWarps * S::stages * S::stage_bytes);
   const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
   const uint32_t ring = smem_addr(smem + warp * S::stages * S::stage_bytes);
   grid_launch_dependents();
@@ -182,36 +182,41 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
   uint32_t qf[D / 16][4];
   float o[D / 8][4], m[2], l[2];
   int limit[2];
-  bool fresh = true;
-  for (int i = 0; i < count; ++i) {
-    if (fresh) {
-      fresh = false;
-      if (threadIdx.x == 0 && p.status) {
-        const int raw = __ldg(p.lengths + at.s);
-        if (raw != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
-      }
-      const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
-      const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = lane / 4 + 8 * u, token = r / part;
-        const bool live = token < tokens;
-        limit[u] = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token0 + token + 1)) : at.q.len;
-        const T* q = static_cast<const T*>(p.q) + (int64_t)(at.q.row0 + token0 + token) * p.q_token +
-                     (int64_t)(at.h / p.blocks * p.group + g0 + r - token * part) * p.q_head + lane % 4 * 2;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][u] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16)) : 0u;
-          qf[kk][u + 2] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16 + 8)) : 0u;
-        }
-        m[u] = -INFINITY;
-        l[u] = 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+  auto start_unit = [&] {
+    if (threadIdx.x == 0 && p.status) {
+      const int raw = __ldg(p.lengths + at.s);
+      if (raw != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
     }
+    const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
+    const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = lane / 4 + 8 * u, token = r / part;
+      const bool live = token < tokens;
+      limit[u] = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token0 + token + 1)) : at.q.len;
+      const T* q = static_cast<const T*>(p.q) + (int64_t)(at.q.row0 + token0 + token) * p.q_token +
+                   (int64_t)(at.h / p.blocks * p.group + g0 + r - token * part) * p.q_head + lane % 4 * 2;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][u] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16)) : 0u;
+        qf[kk][u + 2] = live ? __ldg(reinterpret_cast<const unsigned int*>(q + kk * 16 + 8)) : 0u;
+      }
+    }
+  };
+  auto clear = [&] {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+  };
+  start_unit();
+  clear();
+  for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(S::stages - 2) : "memory");
     __syncwarp();
     issue();   // into the stage read last time round
@@ -284,68 +289,64 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
     ++t;
     if (t < at.tiles && i + 1 < count) continue;
 
-    // The unit's end, or the run's: merge the warps' parts.
+    // The unit's end, or the run's: merge the warps' parts, with the next unit's queries on their way.
     const bool whole = (segment || place.t == 0) && t == at.tiles;
+    const bool ends_first = segment == 0 && !whole && t == at.tiles;
     const int slot = 2 * cta + (segment ? 1 : 0);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      if (lane % 4 == 0) {
-        s_m[warp][lane / 4 + 8 * u] = m[u];
-        s_l[warp][lane / 4 + 8 * u] = l[u];
-      }
+    const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
+    const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+    const int row0 = at.q.row0 + token0, head0 = at.h / p.blocks * p.group + g0;
+    if (i + 1 < count) {
+      at.next(p);
+      start_unit();
     }
-    __syncthreads();
+    // Each warp leaves its part in the stage that it has just read, which is not loaded again before the second barrier.
+    float* mine = reinterpret_cast<float*>(smem + (warp * S::stages + i % S::stages) * S::stage_bytes);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = lane / 4 + 8 * u;
-      float now = s_m[0][r];
-#pragma unroll
-      for (int x = 1; x < kWarps; ++x) now = fmaxf(now, s_m[x][r]);
-      const float f = m[u] == now ? 1.f : exp2_approx(m[u] - now);
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        o[d][2 * u] *= f;
-        o[d][2 * u + 1] *= f;
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      if (lane % 4 == 0) {
+        s_m[warp][r] = m[u];
+        s_l[warp][r] = l[u];
       }
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+        *reinterpret_cast<float2*>(mine + r * S::merge_stride + d * 8 + lane % 4 * 2) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
     }
-    // One row and four of its columns a thread, 32 columns a round.
+    __syncthreads();
+    // One row and four of every 32 columns a thread.
     const int r = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
-    float top_r = s_m[0][r], sum_r = 0.f;
+    float top_r = s_m[0][r], sum_r = 0.f, f[kWarps];
 #pragma unroll
     for (int x = 1; x < kWarps; ++x) top_r = fmaxf(top_r, s_m[x][r]);
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x)
-      sum_r += s_m[x][r] == top_r ? s_l[x][r] : s_l[x][r] * exp2_approx(s_m[x][r] - top_r);
-    const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
-    const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
+    for (int x = 0; x < kWarps; ++x) {
+      f[x] = s_m[x][r] == top_r ? 1.f : exp2_approx(s_m[x][r] - top_r);
+      sum_r += s_l[x][r] * f[x];
+    }
     const bool live = r < tokens * part;
-    const int64_t out_row = (int64_t)(at.q.row0 + token0 + r / part) * p.q_heads + at.h / p.blocks * p.group + g0 + r % part;
+    const int64_t out_row = (int64_t)(row0 + r / part) * p.q_heads + head0 + r % part;
     const float inverse = sum_r == 0.f ? 0.f : 1.f / sum_r;
 #pragma unroll
-    for (int round = 0; round < D / 32; ++round) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          *reinterpret_cast<float2*>(merge + (warp * kRows + lane / 4 + 8 * u) * S::merge_stride + d * 8 + lane % 4 * 2) =
-              make_float2(o[round * 4 + d][2 * u], o[round * 4 + d][2 * u + 1]);
-      __syncthreads();
+    for (int k = 0; k < D / 32; ++k) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < kWarps; ++x) {
-        const float4 f = *reinterpret_cast<const float4*>(merge + (x * kRows + r) * S::merge_stride + c);
-        sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+        const float4 v = *reinterpret_cast<const float4*>(smem + (x * S::stages + i % S::stages) * S::stage_bytes +
+                                                          (r * S::merge_stride + k * 32 + c) * 4);
+        sum.x = fmaf(v.x, f[x], sum.x); sum.y = fmaf(v.y, f[x], sum.y);
+        sum.z = fmaf(v.z, f[x], sum.z); sum.w = fmaf(v.w, f[x], sum.w);
       }
       if (!whole) {
-        *reinterpret_cast<float4*>(p.partial_o + ((int64_t)slot * p.rows + r) * D + round * 32 + c) = sum;
+        *reinterpret_cast<float4*>(p.partial_o + ((int64_t)slot * p.rows + r) * D + k * 32 + c) = sum;
       } else if (live) {
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + round * 32 + c) =
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + k * 32 + c) =
             make_uint2(Half<T>::pack(sum.x * inverse, sum.y * inverse), Half<T>::pack(sum.z * inverse, sum.w * inverse));
       }
-      __syncthreads();
     }
+    __syncthreads();
     if (threadIdx.x % 8 == 0) {
       if (!whole) {
         p.partial_ml[(int64_t)slot * p.rows + r] = make_float2(top_r, sum_r);
@@ -353,13 +354,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_rows_kernel(const Pa
         p.lse[out_row] = sum_r == 0.f ? -INFINITY : (top_r - Half<T>::shift + log2f(sum_r)) * 0.69314718056f;
       }
     }
-    if (threadIdx.x == 0 && segment == 0 && !whole && t == at.tiles)
-      p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + token0, tokens,
-                         at.h / p.blocks * p.group + g0, part, 0};
+    if (threadIdx.x == 0 && ends_first)
+      p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, row0, tokens, head0, part, 0};
     ++segment;
     t = 0;
-    at.next(p);
-    fresh = true;
+    clear();
   }
 }
 
@@ -463,7 +462,7 @@ struct Division {
   int group_part, blocks, unit_tokens, tile_tokens, tile_rows, rows, ctas, min_tiles;
 };
 
-int divide(int tokens, int sequences, int group, int max_query, bool chunk_fits, Division* d) {
+int divide(int tokens, int sequences, int group, int dim, int max_query, bool chunk_fits, Division* d) {
   int sms = 0;
   if (const int rc = sm_count(&sms)) return rc;
   // Rows for each key: of the longest chunk where the caller knows it, else of the mean one.
@@ -483,7 +482,7 @@ int divide(int tokens, int sequences, int group, int max_query, bool chunk_fits,
     d->blocks = (group + kRows - 1) / kRows;
     d->unit_tokens = d->tile_tokens = kRows / d->group_part;
     d->tile_rows = d->rows = kRows;
-    d->ctas = sms * kCtasPerSm;
+    d->ctas = sms * (dim == 64 ? Shape<64>::ctas_per_sm : dim == 96 ? Shape<96>::ctas_per_sm : Shape<128>::ctas_per_sm);
     d->min_tiles = 2;
   }
   return SVX_OK;
@@ -527,7 +526,7 @@ extern "C" size_t svx_paged_attention_workspace_bytes(int tokens, int sequences,
                                                       int max_query) {
   if (sequences < 0 || paged::check_attention(tokens, q_heads, kv_heads, dim)) return 0;
   paged::Division d;
-  if (paged::divide(tokens, sequences, q_heads / kv_heads, max_query, true, &d)) return 0;
+  if (paged::divide(tokens, sequences, q_heads / kv_heads, dim, max_query, true, &d)) return 0;
   return paged::workspace_bytes(d, dim);
 }
 
@@ -550,7 +549,7 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   // The form for many rows reads through tensor maps, whose strides are positive and whose coordinates have 32 bits; the
   // other one takes everything, and less workspace.
   const bool fits = q_token_stride > 0 && q_head_stride > 0 && (int64_t)cache->pages * cache->kv_heads < INT32_MAX;
-  if (const int rc = paged::divide(tokens, cache->sequences, q_heads / cache->kv_heads, max_query, fits, &d)) return rc;
+  if (const int rc = paged::divide(tokens, cache->sequences, q_heads / cache->kv_heads, cache->dim, max_query, fits, &d)) return rc;
   paged::Params p{};
   p.q = q;
   p.q_token = q_token_stride;
