@@ -362,19 +362,17 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kern
   }
 }
 
-// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, rows from
-// y * 8 / kWarpsRow on, kWarpsRow warps a row that share its parts. Reads the partial sums once (they are in L2); a chunk's
-// unit has few parts and many rows, a single token's has few rows and up to a part for every CTA.
-template <typename T, int D, int kWarpsRow>
+// Joins a unit's parts: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m). Block (c, y): the unit that CTA c ended, rows 2 y and
+// 2 y + 1, four warps a row that share its parts (up to one for every CTA). Reads the partial sums once; they are in L2.
+template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   grid_dependency_wait();
   const Join join = p.join[blockIdx.x];
   if (!join.parts) return;
-  constexpr int rows = 8 / kWarpsRow;
+  constexpr int kWarpsRow = 4, rows = 8 / kWarpsRow;
   const int warp = warp_id(), lane = lane_id(), share = warp % kWarpsRow;
-  const int r = blockIdx.y * rows + warp / kWarpsRow, in_tile = r % p.tile_rows;
-  const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
-  const bool live = in_tile < p.tile_tokens * join.group && token < join.tokens;
+  const int r = blockIdx.y * rows + warp / kWarpsRow, token = r / join.group;
+  const bool live = token < join.tokens;
   auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)) * p.rows + r; };
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float top = -INFINITY, total = 0.f;
@@ -407,28 +405,26 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
       }
     }
   }
-  if constexpr (kWarpsRow > 1) {
-    __shared__ float4 s_o[8][32];
-    __shared__ float2 s_ml[8];
-    s_o[warp][lane] = sum;
-    if (lane == 0) s_ml[warp] = make_float2(top, total);
-    __syncthreads();
-    if (share) return;
+  __shared__ float4 s_o[8][32];
+  __shared__ float2 s_ml[8];
+  s_o[warp][lane] = sum;
+  if (lane == 0) s_ml[warp] = make_float2(top, total);
+  __syncthreads();
+  if (share) return;
 #pragma unroll
-    for (int x = 1; x < kWarpsRow; ++x) {
-      const float2 other = s_ml[warp + x];
-      const float4 v = s_o[warp + x][lane];
-      const float now = fmaxf(top, other.x);
-      const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
-      total = total * f + other.y * g;
-      sum.x = sum.x * f + v.x * g; sum.y = sum.y * f + v.y * g;
-      sum.z = sum.z * f + v.z * g; sum.w = sum.w * f + v.w * g;
-      top = now;
-    }
+  for (int x = 1; x < kWarpsRow; ++x) {
+    const float2 other = s_ml[warp + x];
+    const float4 v = s_o[warp + x][lane];
+    const float now = fmaxf(top, other.x);
+    const float f = top == now ? 1.f : exp2_approx(top - now), g = other.x == now ? 1.f : exp2_approx(other.x - now);
+    total = total * f + other.y * g;
+    sum.x = sum.x * f + v.x * g; sum.y = sum.y * f + v.y * g;
+    sum.z = sum.z * f + v.z * g; sum.w = sum.w * f + v.w * g;
+    top = now;
   }
   if (!live) return;
   const float inverse = total == 0.f ? 0.f : 1.f / total;
-  const int64_t out_row = (int64_t)(join.row + token) * p.q_heads + join.head + in_tile % join.group;
+  const int64_t out_row = (int64_t)(join.row + token) * p.q_heads + join.head + r % join.group;
   if (lane < D / 4)
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + 4 * lane) =
         make_uint2(Half<T>::pack(sum.x * inverse, sum.y * inverse), Half<T>::pack(sum.z * inverse, sum.w * inverse));
@@ -489,16 +485,15 @@ int divide(int tokens, int sequences, int group, int dim, int max_query, bool ch
 }
 
 size_t workspace_bytes(const Division& d, int dim) {
-  return (size_t)d.ctas * (sizeof(Join) + 2 * (size_t)d.rows * (dim * sizeof(float) + sizeof(float2)));
+  const size_t rows = 2 * (size_t)d.rows + (d.chunk ? 128 : 0);
+  return (size_t)d.ctas * (sizeof(Join) + rows * (dim * sizeof(float) + sizeof(float2)));
 }
 
 template <typename T, int D>
 int launch_all(const Params& p, const Division& d, int dtype, cudaStream_t stream) {
-  const int rc = d.chunk ? chunk_launch(p, dtype, D, d.ctas, stream) : few_rows_launch<T, D>(p, d.ctas, stream);
-  if (rc) return rc;
-  if (d.chunk)
-    return launch_dependent("join_kernel", join_kernel<T, D, 1>, dim3(d.ctas, d.rows / 8), dim3(256), 0, stream, p);
-  return launch_dependent("join_kernel", join_kernel<T, D, 4>, dim3(d.ctas, d.rows / 2), dim3(256), 0, stream, p);
+  if (d.chunk) return chunk_launch(p, dtype, D, d.ctas, stream);
+  if (const int rc = few_rows_launch<T, D>(p, d.ctas, stream)) return rc;
+  return launch_dependent("join_kernel", join_kernel<T, D>, dim3(d.ctas, d.rows / 2), dim3(256), 0, stream, p);
 }
 
 template <typename T>
@@ -562,10 +557,12 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   p.out = out;
   p.lse = lse;
   p.status = cache->status;
-  const size_t slots = 2 * (size_t)d.ctas * d.rows;
+  const size_t rows = 2 * (size_t)d.ctas * d.rows, split_rows = d.chunk ? 128 * (size_t)d.ctas : 0;
   p.partial_o = static_cast<float*>(workspace);
-  p.partial_ml = reinterpret_cast<float2*>(p.partial_o + slots * cache->dim);
-  p.join = reinterpret_cast<paged::Join*>(p.partial_ml + slots);
+  p.split_o = p.partial_o + rows * cache->dim;
+  p.partial_ml = reinterpret_cast<float2*>(p.split_o + split_rows * cache->dim);
+  p.split_ml = p.partial_ml + rows;
+  p.join = reinterpret_cast<paged::Join*>(p.split_ml + split_rows);
   p.tokens = tokens;
   p.sequences = cache->sequences;
   p.q_heads = q_heads;

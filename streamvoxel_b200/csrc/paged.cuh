@@ -22,9 +22,14 @@ struct Params {
   void* out;                 // [tokens][q_heads][dim]
   float* lse;                // [tokens][q_heads] or null
   uint32_t* status;          // [sequences] or null
-  float* partial_o;          // [2 ctas][rows][dim]: unnormalised sums of a CTA's first and last unit where it has
-  float2* partial_ml;        // [2 ctas][rows]: only a part of it; their exponent bases and sums of exponentials
-  Join* join;         // [ctas]: the unit that each CTA ends for others
+  // Unnormalised sums of a CTA's first and last unit where it has only a part of it: [2 ctas][rows][dim] (few rows), or
+  // [2 ctas][dim / 4][rows] groups of four columns (many rows); their exponent bases and sums of exponentials
+  // [2 ctas][rows]. split_*: the second chain's, of a query tile that both share (many rows), for 128 rows of each CTA.
+  float* partial_o;
+  float2* partial_ml;
+  float* split_o;
+  float2* split_ml;
+  Join* join;                // [ctas]: the unit that each CTA ends for others
   int tokens, sequences, q_heads, kv_heads, group, page_shift, pages, table_width, causal;
   float scale_log2;
   int unit_tokens;           // tokens of a unit
@@ -109,7 +114,7 @@ struct Place {
 };
 
 struct PlanShared {
-  int64_t warp_tiles[16], warp_units[16];   // of at most 512 threads
+  int64_t warp_tiles[20], warp_units[20];   // of at most 640 threads
   Place place;
 };
 
@@ -216,9 +221,9 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
   block_scan<kThreads>(tiles, units, sh, &before, &units_before, &total, &units_total);
   const int64_t each = max((int64_t)p.min_tiles, (total + ctas - 1) / ctas);
   int waves = 0;
-  // The last wave and the rest stay for the runs. A step of `ctas` units reads the sequences that it passes, so they are
-  // not to be many.
-  if (kWaves && units_total >= 2 * (int64_t)ctas && units_total >= 16 * (int64_t)p.sequences)
+  // The last wave and the rest stay for the runs. A step of `ctas` units reads every sequence that it passes, one after the
+  // other, so they are not to be many.
+  if (kWaves && units_total >= 2 * (int64_t)ctas && units_total >= 64 * (int64_t)p.sequences)
     waves = (int)min(units_total / ctas - 1, (int64_t)1 << 20);
   int64_t begin = min(total, each * c), end = min(total, begin + each);
   if (kWaves && waves) {

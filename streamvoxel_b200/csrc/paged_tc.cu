@@ -25,8 +25,12 @@
 // issuing. Warps 4-7 and 8-11 run the tiles' softmax, one row a thread. The exponent base is raised lazily (only when a
 // row's maximum grows by more than 8 in log2 units), a part of the exponentials is evaluated on the FMA pipe; weights are
 // rounded to the cache's type for P V and summed unrounded.
-// A query tile without tokens (the second of a short chunk) is skipped by its chain, and a warp without live rows
-// skips the arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
+// A unit with one query tile (a short chunk, or a single token among chunks) is run by both chains: each takes every
+// second key tile, and the second hands its sums to the first through memory. A warp without live rows skips the
+// arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
+//
+// (Two threads a row, 16 softmax warps instead of eight, took longer: 2,100 cycles a tile against 1,740. All warps of a
+// scheduler reach their exponentials together, so more warps only lengthen that phase.)
 #include <math.h>
 
 #include "common.cuh"
@@ -56,9 +60,10 @@ template <int D> struct Tiles {
   static constexpr int atoms = (D + 63) / 64;             // 128-byte pieces of a row
   static constexpr uint32_t q_atom = TQ * 128, q_bytes = atoms * q_atom;
   static constexpr uint32_t k_atom = TK * 128, k_bytes = atoms * k_atom;
-  static constexpr int stages = atoms == 2 ? 5 : 10;
-  static constexpr int bars = 2 + 4 * stages + 1 + 12;
-  static constexpr size_t smem = 1024 + 2 * q_bytes + 2 * stages * k_bytes + bars * 8 + 16;
+  static constexpr int stages = atoms == 2 ? 4 : 8;
+  static constexpr uint32_t out_bytes = 8 * 4096;         // 32 rows x 128 bytes of each softmax warp, on their way out
+  static constexpr int bars = 2 + 4 * stages + 1 + 15;
+  static constexpr size_t smem = 1024 + 2 * q_bytes + 2 * stages * k_bytes + out_bytes + bars * 8 + 16;
 };
 
 struct Maps {
@@ -219,6 +224,20 @@ struct Walk {
   }
 };
 
+// The key tiles of a unit that chain i takes: all of them for its own query tile, or every second one where the unit has
+// one query tile. Every chain passes every tile of the rings in order, and hands the others' back: a barrier whose phases
+// were not all waited for could be taken a phase too early.
+struct Share {
+  bool split;
+  int count;
+  __device__ __forceinline__ Share(const Params& p, const Walk& w, int i, int tile_tokens) {
+    split = w.at.q.n - w.at.j * p.unit_tokens <= tile_tokens;
+    count = split ? (w.t1 - w.t0 - i + 1) / 2 : w.t1 - w.t0;
+  }
+  __device__ __forceinline__ bool mine(int i, int t) const { return !split || (t & 1) == i; }
+  __device__ __forceinline__ int tile(int i, int u) const { return split ? 2 * u + i : u; }
+};
+
 // Live query tiles of a unit (tile_tokens tokens each).
 __device__ __forceinline__ int live_tiles(const Params& p, const Cursor& at, int tile_tokens) {
   return at.q.n - at.j * p.unit_tokens > tile_tokens ? 2 : 1;
@@ -234,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint8_t* sq = smem;
   uint8_t* sk = sq + 2 * C::q_bytes;
   uint8_t* sv = sk + C::stages * C::k_bytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sv + C::stages * C::k_bytes);
+  uint8_t* so = sv + C::stages * C::k_bytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(so + C::out_bytes);
   uint64_t* q_empty = q_full + 1;             // both chains are past their last S of a unit
   uint64_t* k_full = q_full + 2;
   uint64_t* k_empty = k_full + C::stages;
@@ -244,6 +264,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint64_t* s_full = v_end + 1;               // per query tile and buffer: S computed
   uint64_t* p_full = s_full + 4;              // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
   uint64_t* pv_done = p_full + 4;             // per query tile and buffer: P V completed
+  uint64_t* split_full = pv_done + 4;         // 4 arrivals: the second chain's sums of a shared query tile are in memory
+  uint64_t* split_free = split_full + 1;      // 4 arrivals: they have been read
+  uint64_t* drained = split_free + 1;         // 4 arrivals: all products issued are done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + C::bars);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
@@ -266,6 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(pv_done + i, 1);
     }
+    mbar_init(split_full, 4);
+    mbar_init(split_free, 4);
+    mbar_init(drained, 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::prefetch_map(&maps.q);
@@ -335,7 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               tc::tma_load_3d_w(dst + a * C::k_atom + b * box * 128, map, a * 64, zb, row, bar);
           }
           if (end) {   // rows past the end may hold anything: zeros, then the tile is complete
-            if (!tc::wait_w(v_end, ends & 1, abort_flag)) { ok = false; break; }
+            if (!tc::wait_w(v_end, ends & 1, abort_flag)) {
+              mbar_wait(v_end, ends & 1);
+              ok = false;
+              break;
+            }
             ++ends;
             const int rows = box - left % box;   // to the end of the box
             for (int e = lane; e < C::atoms * rows * 8; e += 32) {
@@ -350,42 +380,47 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
           else if (w.more()) z = look_up(w.at, w.t0);
         }
       }
-      if (!ok)   // loads in flight end before the block does
-        for (int u = max(0, g - C::stages); u < g; ++u) mbar_wait(full + u % C::stages, (u / C::stages) & 1);
+      // Loads in flight end before the block does, also where an abort leaves nothing that waits for them.
+      for (int u = max(0, g - C::stages); u < g; ++u) mbar_wait(full + u % C::stages, (u / C::stages) & 1);
+      if (!is_v && w.units) mbar_wait(q_full, (w.units - 1) & 1);
     } else {   // warp 1: scores of query tile 0; warp 3: of query tile 1
       const int i = warp == 1 ? 0 : 1;
       constexpr uint32_t idesc = descriptor(K::format, TQ, TK, false);
-      const uint32_t qa = smem_addr(sq + i * C::q_bytes), d = tmem + S_COL + 128 * i;
+      const uint32_t d = tmem + S_COL + 128 * i;
       int g = 0, n = 0;   // tiles of the ring and of this chain
       bool ok = true;
       for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
-        const bool idle = i >= live_tiles(p, w.at, tile_tokens);   // no rows: hand the tiles back
-        if (!idle && !tc::wait_w(q_full, w.units & 1, abort_flag)) { ok = false; break; }
-        for (int t = w.t0; t < w.t1; ++t, ++g) {
+        const Share share(p, w, i, tile_tokens);
+        const uint64_t q = tc::sw128_desc(smem_addr(sq + (share.split ? 0 : i) * C::q_bytes));
+        if (!tc::wait_w(q_full, w.units & 1, abort_flag)) { ok = false; break; }
+        for (int t = 0; t < w.t1 - w.t0; ++t, ++g) {
           const int s = g % C::stages;
           ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
           if (!ok) break;
-          if (idle) {
+          if (!share.mine(i, t)) {
             if (lane == 0) tc::mbar_arrive(k_empty + s);
             continue;
           }
           // S(n) goes where P(n - 2) was
-          if (n >= 2 && !__all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2))) { ok = false; break; }
+          ok = n < 2 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2));
+          if (!ok) break;
           tc::fence_after();
-          issue_scores<D>(d + 64 * (n & 1), tc::sw128_desc(qa), tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
+          issue_scores<D>(d + 64 * (n & 1), q, tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
                           s_full + 2 * i + (n & 1), k_empty + s);
           ++n;
         }
         if (!ok) break;
-        if (!idle) tc::commit_w(q_empty);
+        if (share.count) tc::commit_w(q_empty);
         else if (lane == 0) tc::mbar_arrive(q_empty);
       }
+      tc::commit_w(drained);
     }
     // Teardown: the TMEM owner frees the columns once all 14 warps are past their last TMEM access.
     tc::fence_before();
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
     if (warp == 1) {
+      mbar_wait(drained, 0);
       tc::fence_after();
       tc::tmem_dealloc(*tmem_slot, TMEM_COLS);
     }
@@ -399,23 +434,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     int g = 0, n = 0;
     bool ok = true;
     for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
-      const bool idle = i >= live_tiles(p, w.at, tile_tokens);
-      for (int t = w.t0; t < w.t1; ++t, ++g) {
+      const Share share(p, w, i, tile_tokens);
+      bool fresh = true;   // a unit's first product starts O afresh
+      for (int t = 0; t < w.t1 - w.t0; ++t, ++g) {
         const int s = g % C::stages;
         ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
         if (!ok) break;
-        if (idle) {
+        if (!share.mine(i, t)) {
           if (lane == 0) tc::mbar_arrive(v_empty + s);
           continue;
         }
         ok = __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
         if (!ok) break;
         tc::fence_after();
-        issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc,
-                     t != w.t0, pv_done + 2 * i + (n & 1), v_empty + s);   // a unit's first product starts O afresh
+        issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc, !fresh,
+                     pv_done + 2 * i + (n & 1), v_empty + s);
+        fresh = false;
         ++n;
       }
     }
+    tc::commit_w(drained);
     tc::fence_before();
     __syncwarp();
     asm volatile("barrier.arrive 1, %0;" ::"n"(kThreads) : "memory");
@@ -426,9 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
   const uint32_t to = tmem + lanes + O_COL + 128 * i;
   const float sl2 = p.scale_log2;
-  const int my_token = i * tile_tokens + row / p.group;
   const bool in_tile = row < tile_tokens * p.group;
-  int n0 = 0;
+  int n0 = 0, splits = 0;
   bool ok = true;
   Walk w(p, place);
   for (; ok && w.more(); w.next(p, place)) {
@@ -436,16 +473,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     if (p.status && threadIdx.x == 128) {
       if (__ldg(p.lengths + at.s) != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
     }
-    if (i >= live_tiles(p, at, tile_tokens)) continue;
-    const int tiles = w.t1 - w.t0, token = at.j * p.unit_tokens + my_token;
+    const Share share(p, w, i, tile_tokens);
+    const int token = at.j * p.unit_tokens + (share.split ? 0 : i * tile_tokens) + row / p.group;
     const bool live = in_tile && token < at.q.n;
     // Keys that this row sees; a dead row's result is not stored.
     const int limit = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token + 1)) : at.q.len;
     const int least = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
     const bool warp_live = least != 0x7fffffff;
     float m_used = -INFINITY, l_run = 0.f;
-    for (int t = 0; t < tiles; ++t) {
-      const int n = n0 + t, buffer = n & 1;
+    for (int u = 0; u < share.count; ++u) {
+      const int n = n0 + u, buffer = n & 1;
       const uint32_t ts = tmem + lanes + S_COL + 128 * i + 64 * buffer;
       if (!buffer_wait(s_full, i, n)) { ok = false; break; }
       if (!warp_live) {
@@ -458,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       tc::ld32(ts, r[0]);
       tc::ld32(ts + 32, r[1]);
       tc::wait_ld();
-      const int key0 = (w.t0 + t) * TK;
+      const int key0 = (w.t0 + share.tile(i, u)) * TK;
       if (key0 + TK > least) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -501,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         packed[j >> 1] = K::pack(e.x, e.y);
       }
       tc::st32(ts, packed);
-      if (any_raise && t >= 1) {   // O holds the products of the earlier tiles once P(t - 1) V(t - 1) is done
+      if (any_raise && u >= 1) {   // O holds the products of the earlier tiles once P(t - 1) V(t - 1) is done
         if (!buffer_wait(pv_done, i, n - 1)) { ok = false; break; }
         tc::fence_after();
 #pragma unroll
@@ -521,44 +558,128 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_full + 2 * i + buffer);
     }
-    if (ok) ok = buffer_wait(pv_done, i, n0 + tiles - 1);
+    if (ok && share.count) ok = buffer_wait(pv_done, i, n0 + share.count - 1);
+    ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     tc::fence_after();
-    n0 += tiles;
+    n0 += share.count;
     const bool whole = w.t0 == 0 && w.t1 == at.tiles;
-    const int64_t slot = (int64_t)(2 * cta + (w.part > 0 ? 1 : 0)) * p.rows + i * TQ + row;
-    const int64_t out_row = (int64_t)(at.q.row0 + token) * p.q_heads + at.h * p.group + row % p.group;
     // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
     // makes the row NaN, as inf - inf does.
-    const bool none = m_used == -INFINITY;
     if (m_used == INFINITY) l_run = __int_as_float(0x7fffffff);
-    if (none) l_run = 0.f;
-    const float factor = none ? 0.f : whole ? 1.f / l_run : 1.f;
-    if (warp_live) {
+    if (m_used == -INFINITY) l_run = 0.f;
+    float factor = m_used == -INFINITY ? 0.f : 1.f, other_factor = 0.f;
+    if (share.split && i == 1) {
+      if (splits >= 1) ok = __all_sync(0xffffffffu, tc::wait(split_free, (splits - 1) & 1, abort_flag));
+      if (!ok) break;
+      if (warp_live) {
+        if (live) p.split_ml[(int64_t)cta * TQ + row] = make_float2(m_used, l_run);
+        float4* dst = reinterpret_cast<float4*>(p.split_o) + (int64_t)cta * TQ * (D / 4) + row;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tc::ld32(to + c * 32, o);
-        tc::wait_ld();
-        if (!live) continue;
-        float f[32];
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tc::ld32(to + c * 32, o);
+          tc::wait_ld();
+          if (live && factor != 0.f) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = none ? 0.f : __uint_as_float(o[j]) * factor;
-        if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * D + c * 32);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            dst[k] = make_uint4(K::pack(f[8 * k], f[8 * k + 1]), K::pack(f[8 * k + 2], f[8 * k + 3]),
-                                K::pack(f[8 * k + 4], f[8 * k + 5]), K::pack(f[8 * k + 6], f[8 * k + 7]));
-        } else {
-          float4* dst = reinterpret_cast<float4*>(p.partial_o + slot * D + c * 32);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) dst[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            for (int k = 0; k < 8; ++k)
+              dst[(c * 8 + k) * TQ] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                                  __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+          }
         }
       }
-      if (live && !whole) p.partial_ml[slot] = make_float2(m_used, l_run);
-      if (live && whole && p.lse)
-        p.lse[out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(split_full);
+      ++splits;
+      continue;
+    }
+    if (share.split) {   // the second chain's sums join the first's
+      ok = __all_sync(0xffffffffu, tc::wait(split_full, splits & 1, abort_flag));
+      if (!ok) break;
+      if (live) {
+        const float2 ml = __ldcg(p.split_ml + (int64_t)cta * TQ + row);
+        const float m_new = max2_nan(m_used, ml.x);
+        other_factor = ml.x == -INFINITY ? 0.f : ml.x == m_new ? 1.f : tc::ex2(ml.x - m_new);
+        factor = m_used == -INFINITY ? 0.f : m_used == m_new ? 1.f : tc::ex2(m_used - m_new);
+        l_run = l_run * factor + ml.y * other_factor;
+        m_used = m_new;
+      }
+    }
+    const bool none = m_used == -INFINITY;
+    const float inverse = !whole ? 1.f : none ? 0.f : 1.f / l_run;
+    if (warp_live) {
+      // Columns [c, c + 32) of this thread's row.
+      auto columns = [&](int c, float (&f)[32]) {
+        uint32_t o[32];
+        tc::ld32(to + c, o);
+        tc::wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = factor == 0.f ? 0.f : __uint_as_float(o[j]) * factor;
+        if (live && other_factor != 0.f) {   // NaN too
+          const float4* src = reinterpret_cast<const float4*>(p.split_o) + (int64_t)cta * TQ * (D / 4) + row;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 x = __ldcg(src + (c / 4 + k) * TQ);
+            f[4 * k] = fmaf(x.x, other_factor, f[4 * k]);
+            f[4 * k + 1] = fmaf(x.y, other_factor, f[4 * k + 1]);
+            f[4 * k + 2] = fmaf(x.z, other_factor, f[4 * k + 2]);
+            f[4 * k + 3] = fmaf(x.w, other_factor, f[4 * k + 3]);
+          }
+        }
+      };
+      if (!whole) {   // neighbouring rows are neighbours in memory
+        const int64_t slot = 2 * cta + (w.part > 0 ? 1 : 0);
+        const int r = (share.split ? 0 : i * TQ) + row;
+        float4* dst = reinterpret_cast<float4*>(p.partial_o) + slot * p.rows * (D / 4) + r;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float f[32];
+          columns(c, f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (live) dst[(c / 4 + k) * p.rows] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+        }
+        if (live) p.partial_ml[slot * p.rows + r] = make_float2(m_used, l_run);
+      } else {   // through shared memory, so that eight lanes write 128 bytes of a row
+        const int64_t row0 = (int64_t)(at.q.row0 + at.j * p.unit_tokens) * p.q_heads + at.h * p.group;
+        const int out_row = live ? (token - at.j * p.unit_tokens) * p.q_heads + row % p.group : -1;
+        uint8_t* mine = so + (warp - 4) * 4096;
+#pragma unroll
+        for (int c = 0; c < D; c += 64) {
+          constexpr int wide = 64;
+          const int pieces = (D - c < wide ? D - c : wide) / 8;   // of 16 bytes a row
+#pragma unroll
+          for (int b = 0; b < pieces / 4; ++b) {
+            float f[32];
+            columns(c + 32 * b, f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(mine + lane * 128 + (((4 * b + k) ^ (lane & 7)) * 16)) =
+                  make_uint4(K::pack(f[8 * k] * inverse, f[8 * k + 1] * inverse),
+                             K::pack(f[8 * k + 2] * inverse, f[8 * k + 3] * inverse),
+                             K::pack(f[8 * k + 4] * inverse, f[8 * k + 5] * inverse),
+                             K::pack(f[8 * k + 6] * inverse, f[8 * k + 7] * inverse));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < pieces; ++k) {
+            const int r = (32 * k + lane) / pieces, piece = lane % pieces;
+            const int to_row = __shfl_sync(0xffffffffu, out_row, r);
+            const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) * 16));
+            if (to_row >= 0)
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + to_row) * D + c + piece * 8) = x;
+          }
+          __syncwarp();
+        }
+        if (live && p.lse)
+          p.lse[row0 + out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
+      }
+    }
+    if (share.split) {
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(split_free);
+      ++splits;
     }
     if (threadIdx.x == 128 && w.part == 0 && !whole && w.t1 == at.tiles)
       p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + at.j * p.unit_tokens,
@@ -576,6 +697,61 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   asm volatile("barrier.arrive 1, %0;" ::"n"(kThreads) : "memory");
 }
 
+// Joins a unit's parts (see join_kernel of the few rows). A warp takes 32 rows and 32 columns: a lane reads its row's
+// columns of every part (neighbouring rows are neighbours in memory) and the warp writes through shared memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const Params p) {
+  __shared__ __align__(16) uint8_t stage[8][32 * 64];
+  grid_dependency_wait();
+  const Join join = p.join[blockIdx.x];
+  if (!join.parts) return;
+  const int warp = warp_id(), lane = lane_id(), task = blockIdx.y * 8 + warp;
+  const int r = task / (D / 32) * 32 + lane, c = task % (D / 32) * 32, in_tile = r % p.tile_rows;
+  const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
+  const bool live = in_tile < p.tile_tokens * join.group && token < join.tokens;
+  if (!__any_sync(0xffffffffu, live)) return;
+  auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)); };
+  float top = -INFINITY, total = 0.f, f[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) f[j] = 0.f;
+  if (live) {
+    for (int i = 0; i < join.parts; ++i) top = fmaxf(top, p.partial_ml[slot(i) * p.rows + r].x);
+    for (int i = 0; i < join.parts; ++i) {
+      const float2 ml = p.partial_ml[slot(i) * p.rows + r];
+      const float4* src = reinterpret_cast<const float4*>(p.partial_o) + slot(i) * p.rows * (D / 4) + c / 4 * p.rows + r;
+      const float x = ml.x == top ? 1.f : tc::ex2(ml.x - top);
+      total = fmaf(ml.y, x, total);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float4 v = src[k * p.rows];
+        f[4 * k] = fmaf(v.x, x, f[4 * k]);
+        f[4 * k + 1] = fmaf(v.y, x, f[4 * k + 1]);
+        f[4 * k + 2] = fmaf(v.z, x, f[4 * k + 2]);
+        f[4 * k + 3] = fmaf(v.w, x, f[4 * k + 3]);
+      }
+    }
+  }
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  const int64_t row0 = (int64_t)join.row * p.q_heads + join.head;
+  const int out_row = live ? token * p.q_heads + in_tile % join.group : -1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(stage[warp] + lane * 64 + ((k ^ (lane & 3)) * 16)) =
+        make_uint4(Kind<T>::pack(f[8 * k] * inverse, f[8 * k + 1] * inverse),
+                   Kind<T>::pack(f[8 * k + 2] * inverse, f[8 * k + 3] * inverse),
+                   Kind<T>::pack(f[8 * k + 4] * inverse, f[8 * k + 5] * inverse),
+                   Kind<T>::pack(f[8 * k + 6] * inverse, f[8 * k + 7] * inverse));
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int q = 8 * k + lane / 4, piece = lane % 4, to_row = __shfl_sync(0xffffffffu, out_row, q);
+    const uint4 x = *reinterpret_cast<const uint4*>(stage[warp] + q * 64 + ((piece ^ (q & 3)) * 16));
+    if (to_row >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + to_row) * D + c + piece * 8) = x;
+  }
+  if (live && c == 0 && p.lse)
+    p.lse[row0 + out_row] = total == 0.f ? -INFINITY : (top - Kind<T>::shift + log2f(total)) * 0.69314718056f;
+}
+
 template <typename T, int D>
 int launch(const Maps& maps, const Params& p, int ctas, cudaStream_t stream) {
   static PerDevice<int> ready;
@@ -585,7 +761,10 @@ int launch(const Maps& maps, const Params& p, int ctas, cudaStream_t stream) {
     return SVX_OK;
   });
   if (rc) return rc;
-  return launch_dependent("chunk_kernel", chunk_kernel<T, D>, dim3(ctas), dim3(kThreads), Tiles<D>::smem, stream, maps, p);
+  if (const int rc = launch_dependent("chunk_kernel", chunk_kernel<T, D>, dim3(ctas), dim3(kThreads), Tiles<D>::smem,
+                                      stream, maps, p))
+    return rc;
+  return launch_dependent("chunk_join_kernel", chunk_join_kernel<T, D>, dim3(ctas, D / 32), dim3(256), 0, stream, p);
 }
 
 }  // namespace
