@@ -468,10 +468,11 @@ int divide(int tokens, int sequences, int group, int dim, int max_query, bool ch
     d->group_part = group;
     d->blocks = 1;
     d->tile_tokens = 128 / group;
-    d->unit_tokens = 2 * d->tile_tokens;
+    const int tiles = query > d->tile_tokens ? 2 : 1;   // query tiles of a unit, and then two or one CTA a SM
+    d->unit_tokens = tiles * d->tile_tokens;
     d->tile_rows = 128;
-    d->rows = 256;
-    d->ctas = sms;
+    d->rows = 128 * tiles;
+    d->ctas = sms * (3 - tiles);
     d->min_tiles = 4;
   } else {
     d->group_part = std::min(group, kRows);
@@ -485,8 +486,7 @@ int divide(int tokens, int sequences, int group, int dim, int max_query, bool ch
 }
 
 size_t workspace_bytes(const Division& d, int dim) {
-  const size_t rows = 2 * (size_t)d.rows + (d.chunk ? 128 : 0);
-  return (size_t)d.ctas * (sizeof(Join) + rows * (dim * sizeof(float) + sizeof(float2)));
+  return (size_t)d.ctas * (sizeof(Join) + 2 * (size_t)d.rows * (dim * sizeof(float) + sizeof(float2)));
 }
 
 template <typename T, int D>
@@ -557,12 +557,10 @@ extern "C" int svx_paged_attention(const svx_paged_cache* cache, const void* q, 
   p.out = out;
   p.lse = lse;
   p.status = cache->status;
-  const size_t rows = 2 * (size_t)d.ctas * d.rows, split_rows = d.chunk ? 128 * (size_t)d.ctas : 0;
+  const size_t rows = 2 * (size_t)d.ctas * d.rows;
   p.partial_o = static_cast<float*>(workspace);
-  p.split_o = p.partial_o + rows * cache->dim;
-  p.partial_ml = reinterpret_cast<float2*>(p.split_o + split_rows * cache->dim);
-  p.split_ml = p.partial_ml + rows;
-  p.join = reinterpret_cast<paged::Join*>(p.split_ml + split_rows);
+  p.partial_ml = reinterpret_cast<float2*>(p.partial_o + rows * cache->dim);
+  p.join = reinterpret_cast<paged::Join*>(p.partial_ml + rows);
   p.tokens = tokens;
   p.sequences = cache->sequences;
   p.q_heads = q_heads;

@@ -24,11 +24,9 @@ struct Params {
   uint32_t* status;          // [sequences] or null
   // Unnormalised sums of a CTA's first and last unit where it has only a part of it: [2 ctas][rows][dim] (few rows), or
   // [2 ctas][dim / 4][rows] groups of four columns (many rows); their exponent bases and sums of exponentials
-  // [2 ctas][rows]. split_*: the second chain's, of a query tile that both share (many rows), for 128 rows of each CTA.
+  // [2 ctas][rows].
   float* partial_o;
   float2* partial_ml;
-  float* split_o;
-  float2* split_ml;
   Join* join;                // [ctas]: the unit that each CTA ends for others
   int tokens, sequences, q_heads, kv_heads, group, page_shift, pages, table_width, causal;
   float scale_log2;

@@ -2,11 +2,12 @@
 //
 // Same mathematics and the same division into equal runs of 64-key tiles as the few-rows form (paged.cu, paged.cuh), for
 // calls with many query rows for each key, which are bound by the products and the softmax's exponentials instead of
-// memory. A unit is two 128-row query tiles of one (sequence, kv head): the rows of a tile are 128 / group tokens with
-// all the query heads of the group, so that a key tile is loaded once for the whole group, and a short chunk still
-// fills the rows of the products.
+// memory. The rows of a 128-row query tile are 128 / group tokens with all the query heads of the group, so that a key tile
+// is loaded once for the whole group, and a short chunk still fills the rows of the products. A unit is two query tiles of
+// one (sequence, kv head), with one CTA a SM; or one, with two CTAs a SM, for calls whose chunks fit a query tile: the
+// two then take different units, and one computes while the other starts or ends its own.
 //
-// A persistent CTA per SM takes its run of the line of tiles. K and V tiles of 64 keys are streamed by TMA through
+// A persistent CTA takes its run of the line of tiles. K and V tiles of 64 keys are streamed by TMA through
 // rings, one box per page (or 64 keys of a larger page), the page ids looked up one tile ahead. Boxes past the
 // sequence's end load nothing and come as zeros; in the box that holds the end, the rows of V past it are zeroed in
 // shared memory before the products see them, so that nothing a page holds past the length (NaN, infinities) reaches
@@ -14,23 +15,22 @@
 // are not multiplied).
 //
 // Tensor memory: two S buffers of each query tile (fp32, tile t in buffer t % 2 at [128 i + 64 (t % 2), +64)) and O_i
-// (fp32 at [256 + 128 i, +D)). The softmax writes P(t) (16-bit pairs) over the first 32 columns of the S buffer that it
-// has read, so S(t + 2) follows P(t) V(t) there, while S(t + 1) is ready before the softmax of tile t is done: the
-// softmax waits for no product but its own tile's. (With one S buffer and P apart the softmax waited 300-450 of the
-// 1,800 cycles of a tile for S: clock stamps.)
+// (fp32, 128 columns each after the S buffers). The softmax writes P(t) (16-bit pairs) over the first 32 columns of the S
+// buffer that it has read, so S(t + 2) follows P(t) V(t) there, while S(t + 1) is ready before the softmax of tile t is
+// done: the softmax waits for no product but its own tile's. (With one S buffer and P apart the softmax waited 300-450 of
+// the 1,800 cycles of a tile for S: clock stamps.)
 //
-// Warp roles (448 threads): warp 0 loads Q and the K ring, warp 2 the V ring; warps 1 and 3 issue the scores of query
-// tiles 0 and 1, warps 12 and 13 their products with V (an issuing warp takes a few hundred cycles for a batch of
-// products and its waits, which one warp a tile could not hide); each of these loops is warp-converged, one elected lane
-// issuing. Warps 4-7 and 8-11 run the tiles' softmax, one row a thread. The exponent base is raised lazily (only when a
-// row's maximum grows by more than 8 in log2 units), a part of the exponentials is evaluated on the FMA pipe; weights are
-// rounded to the cache's type for P V and summed unrounded.
-// A unit with one query tile (a short chunk, or a single token among chunks) is run by both chains: each takes every
-// second key tile, and the second hands its sums to the first through memory. A warp without live rows skips the
-// arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
+// Warp roles: warp 0 loads Q and the K ring, warp 2 the V ring; a warp for each query tile issues its scores and another
+// its products with V (an issuing warp takes a few hundred cycles for a batch of products and its waits, which one warp a
+// tile could not hide); each of these loops is warp-converged, one elected lane issuing. Four warps a query tile run its
+// softmax, one row a thread. The exponent base is raised lazily (only when a row's maximum grows by more than 8 in log2
+// units), a part of the exponentials is evaluated on the FMA pipe; weights are rounded to the cache's type for P V and
+// summed unrounded. A query tile without tokens (the second of a unit's) is skipped by its chain, and a warp without live
+// rows skips the arithmetic. Every wait is bounded; a timeout sets SVX_STATUS_WAIT_TIMEOUT and skips the rest.
 //
-// (Two threads a row, 16 softmax warps instead of eight, took longer: 2,100 cycles a tile against 1,740. All warps of a
-// scheduler reach their exponentials together, so more warps only lengthen that phase.)
+// Built, measured and not kept: two threads a row (16 softmax warps; 2,100 cycles a tile against 1,740: the warps of a
+// scheduler reach their exponentials together), and both chains on one query tile, every second key tile each (handing the
+// sums over took 4 to 7 us a unit).
 #include <math.h>
 
 #include "common.cuh"
@@ -52,19 +52,41 @@ namespace paged {
 namespace {
 
 constexpr int TQ = 128, TK = kTile;
-constexpr int kThreads = 448;
-constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t S_COL = 0, O_COL = 256;   // + 128 i
 
-template <int D> struct Tiles {
+template <int D, int kChains> struct Tiles {
+  static constexpr int threads = kChains == 2 ? 448 : 256;
+  static constexpr uint32_t tmem_cols = 256 * kChains, s_col = 0, o_col = 128 * kChains;   // + 128 i
   static constexpr int atoms = (D + 63) / 64;             // 128-byte pieces of a row
   static constexpr uint32_t q_atom = TQ * 128, q_bytes = atoms * q_atom;
   static constexpr uint32_t k_atom = TK * 128, k_bytes = atoms * k_atom;
-  static constexpr int stages = atoms == 2 ? 4 : 8;
-  static constexpr uint32_t out_bytes = 8 * 4096;         // 32 rows x 128 bytes of each softmax warp, on their way out
-  static constexpr int bars = 2 + 4 * stages + 1 + 15;
-  static constexpr size_t smem = 1024 + 2 * q_bytes + 2 * stages * k_bytes + out_bytes + bars * 8 + 16;
+  static constexpr int stages = kChains == 2 ? (atoms == 2 ? 4 : 8) : (atoms == 2 ? 2 : 4);
+  static constexpr int out_cols = 32 * kChains;           // columns of each softmax warp's 32 rows on their way out
+  static constexpr uint32_t out_row = out_cols * 2, out_bytes = kChains * 4 * 32 * out_row;
+  static constexpr int bars = 2 + 4 * stages + 1 + 6 * kChains + 1;
+  static constexpr size_t smem = 1024 + kChains * q_bytes + 2 * stages * k_bytes + out_bytes + bars * 8 + 16;
 };
+
+// Bounded waits (two to three seconds) that give up as soon as another role of the CTA raised `abort`. The clock is read
+// between batches of polls: a wait of this kernel is often a few hundred cycles, and %globaltimer takes about as long.
+constexpr long long kWaitCycles = 4000000000ll;
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (clock64() - start > kWaitCycles) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+  return __all_sync(0xffffffffu, wait(bar, parity, abort));
+}
 
 struct Maps {
   CUtensorMap q, k, v;
@@ -145,6 +167,14 @@ __device__ __forceinline__ void issue_values(uint32_t d, uint32_t p, uint64_t v,
 #undef SVX_SS_STEP
 #undef SVX_COMMIT
 
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
 // max(a, b, c), NaN where any of them is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
@@ -224,34 +254,21 @@ struct Walk {
   }
 };
 
-// The key tiles of a unit that chain i takes: all of them for its own query tile, or every second one where the unit has
-// one query tile. Every chain passes every tile of the rings in order, and hands the others' back: a barrier whose phases
-// were not all waited for could be taken a phase too early.
-struct Share {
-  bool split;
-  int count;
-  __device__ __forceinline__ Share(const Params& p, const Walk& w, int i, int tile_tokens) {
-    split = w.at.q.n - w.at.j * p.unit_tokens <= tile_tokens;
-    count = split ? (w.t1 - w.t0 - i + 1) / 2 : w.t1 - w.t0;
-  }
-  __device__ __forceinline__ bool mine(int i, int t) const { return !split || (t & 1) == i; }
-  __device__ __forceinline__ int tile(int i, int u) const { return split ? 2 * u + i : u; }
-};
-
 // Live query tiles of a unit (tile_tokens tokens each).
 __device__ __forceinline__ int live_tiles(const Params& p, const Cursor& at, int tile_tokens) {
   return at.q.n - at.j * p.unit_tokens > tile_tokens ? 2 : 1;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constant__ Maps maps, const Params p) {
-  using C = Tiles<D>;
+template <typename T, int D, int kChains>
+__global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains) chunk_kernel(const __grid_constant__ Maps maps, const Params p) {
+  using C = Tiles<D, kChains>;
   using K = Kind<T>;
+  constexpr int kThreads = C::threads;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PlanShared plan_shared;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
-  uint8_t* sk = sq + 2 * C::q_bytes;
+  uint8_t* sk = sq + kChains * C::q_bytes;
   uint8_t* sv = sk + C::stages * C::k_bytes;
   uint8_t* so = sv + C::stages * C::k_bytes;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(so + C::out_bytes);
@@ -262,45 +279,41 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   uint64_t* v_empty = v_full + C::stages;
   uint64_t* v_end = v_empty + C::stages;      // the load of a V tile that holds the sequence's end
   uint64_t* s_full = v_end + 1;               // per query tile and buffer: S computed
-  uint64_t* p_full = s_full + 4;              // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
-  uint64_t* pv_done = p_full + 4;             // per query tile and buffer: P V completed
-  uint64_t* split_full = pv_done + 4;         // 4 arrivals: the second chain's sums of a shared query tile are in memory
-  uint64_t* split_free = split_full + 1;      // 4 arrivals: they have been read
-  uint64_t* drained = split_free + 1;         // 4 arrivals: all products issued are done
+  uint64_t* p_full = s_full + 2 * kChains;              // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
+  uint64_t* pv_done = p_full + 2 * kChains;   // per query tile and buffer: P V completed
+  uint64_t* drained = pv_done + 2 * kChains;  // 2 arrivals a chain: all products issued are done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + C::bars);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   // Tile n of a chain (counted over the CTA's whole run) uses buffer n % 2, whose barriers are in phase n / 2. With one
   // barrier for both buffers a wait could find the phase two tiles back and take it for its own.
   auto buffer_wait = [&](uint64_t* bars, int i, int n) {
-    return tc::wait(bars + 2 * i + (n & 1), (n >> 1) & 1, abort_flag);
+    return wait(bars + 2 * i + (n & 1), (n >> 1) & 1, abort_flag);
   };
   const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
   const int tile_tokens = p.tile_tokens;
   grid_launch_dependents();
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
+    mbar_init(q_empty, kChains);
     for (int i = 0; i < C::stages; ++i) {
-      mbar_init(k_full + i, 1); mbar_init(k_empty + i, 2);
-      mbar_init(v_full + i, 1); mbar_init(v_empty + i, 2);
+      mbar_init(k_full + i, 1); mbar_init(k_empty + i, kChains);
+      mbar_init(v_full + i, 1); mbar_init(v_empty + i, kChains);
     }
     mbar_init(v_end, 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2 * kChains; ++i) {
       mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); mbar_init(pv_done + i, 1);
     }
-    mbar_init(split_full, 4);
-    mbar_init(split_free, 4);
-    mbar_init(drained, 4);
+    mbar_init(drained, 2 * kChains);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tc::prefetch_map(&maps.q);
     tc::prefetch_map(&maps.k);
     tc::prefetch_map(&maps.v);
   }
-  if (warp == 1) tc::tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp == 1) tc::tmem_alloc(tmem_slot, C::tmem_cols);
   grid_dependency_wait();
-  plan<kThreads, true>(p, cta, gridDim.x, plan_shared, reinterpret_cast<int64_t*>(smem));   // before the tiles are loaded
+  plan<kThreads, kChains == 2>(p, cta, gridDim.x, plan_shared, reinterpret_cast<int64_t*>(smem));   // before the tiles are loaded
   if (threadIdx.x == 0) p.join[cta].parts = 0;
   tc::fence_async_smem();
   tc::fence_before();
@@ -310,6 +323,65 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
   const Place& place = plan_shared.place;
   const int page_mask = (1 << p.page_shift) - 1, box = min(TK, 1 << p.page_shift), boxes = TK / box;
   const int nowhere = p.pages * p.kv_heads;   // a coordinate past the pool: loads zeros
+
+  // A chain without live rows in a unit hands its tiles back.
+  auto idle = [&](const Walk& w, int i) { return i >= live_tiles(p, w.at, tile_tokens); };
+  auto issue_all_scores = [&](int i) {
+    constexpr uint32_t idesc = descriptor(K::format, TQ, TK, false);
+    const uint32_t d = tmem + C::s_col + 128 * i;
+    const uint64_t q = tc::sw128_desc(smem_addr(sq + i * C::q_bytes));
+    int g = 0, n = 0;   // tiles of the ring and of this chain
+    bool ok = true;
+    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
+      const bool none = idle(w, i);
+      if (!wait_w(q_full, w.units & 1, abort_flag)) break;
+      for (int t = w.t0; t < w.t1; ++t, ++g) {
+        const int s = g % C::stages;
+        ok = wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
+        if (!ok) break;
+        if (none) {
+          if (lane == 0) tc::mbar_arrive(k_empty + s);
+          continue;
+        }
+        // S(n) goes where P(n - 2) was
+        ok = n < 2 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2));
+        if (!ok) break;
+        tc::fence_after();
+        issue_scores<D>(d + 64 * (n & 1), q, tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
+                        s_full + 2 * i + (n & 1), k_empty + s);
+        ++n;
+      }
+      if (!ok) break;
+      if (!none) tc::commit_w(q_empty);
+      else if (lane == 0) tc::mbar_arrive(q_empty);
+    }
+    tc::commit_w(drained);
+  };
+  auto issue_all_values = [&](int i) {
+    constexpr uint32_t idesc = descriptor(K::format, TQ, D, true);
+    const uint32_t d = tmem + C::o_col + 128 * i, a = tmem + C::s_col + 128 * i;
+    int g = 0, n = 0;
+    bool ok = true;
+    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
+      const bool none = idle(w, i);
+      for (int t = w.t0; t < w.t1; ++t, ++g) {
+        const int s = g % C::stages;
+        ok = wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
+        if (!ok) break;
+        if (none) {
+          if (lane == 0) tc::mbar_arrive(v_empty + s);
+          continue;
+        }
+        ok = __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
+        if (!ok) break;
+        tc::fence_after();
+        issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc, t != w.t0,
+                     pv_done + 2 * i + (n & 1), v_empty + s);   // a unit's first product starts O afresh
+        ++n;
+      }
+    }
+    tc::commit_w(drained);
+  };
 
   if (warp < 4) {
     if (warp == 0 || warp == 2) {   // K with Q, and V
@@ -335,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       int z = w.more() ? look_up(w.at, w.t0) : nowhere;
       while (ok && w.more()) {
         if (!is_v) {
-          if (w.units && !tc::wait_w(q_empty, (w.units - 1) & 1, abort_flag)) { ok = false; break; }
-          const int nq = live_tiles(p, w.at, tile_tokens);
+          if (w.units && !wait_w(q_empty, (w.units - 1) & 1, abort_flag)) { ok = false; break; }
+          const int nq = kChains == 2 ? live_tiles(p, w.at, tile_tokens) : 1;
           const uint32_t tile_bytes = C::atoms * 128 * tile_tokens * p.group;
           tc::expect_tx_w(q_full, nq * tile_bytes);
           for (int i = 0; i < nq; ++i)
@@ -349,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         w.next(p, place);
         for (int t = t0; t < t1; ++t, ++g) {
           const int s = g % C::stages;
-          if (g >= C::stages && !tc::wait_w(empty + s, (g / C::stages - 1) & 1, abort_flag)) { ok = false; break; }
+          if (g >= C::stages && !wait_w(empty + s, (g / C::stages - 1) & 1, abort_flag)) { ok = false; break; }
           const int left = at.q.len - t * TK;   // keys of the sequence from this tile on
           const bool end = is_v && left > 0 && left < TK && left % box != 0;
           uint64_t* bar = end ? v_end : full + s;
@@ -361,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
               tc::tma_load_3d_w(dst + a * C::k_atom + b * box * 128, map, a * 64, zb, row, bar);
           }
           if (end) {   // rows past the end may hold anything: zeros, then the tile is complete
-            if (!tc::wait_w(v_end, ends & 1, abort_flag)) {
+            if (!wait_w(v_end, ends & 1, abort_flag)) {
               mbar_wait(v_end, ends & 1);
               ok = false;
               break;
@@ -383,77 +455,25 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       // Loads in flight end before the block does, also where an abort leaves nothing that waits for them.
       for (int u = max(0, g - C::stages); u < g; ++u) mbar_wait(full + u % C::stages, (u / C::stages) & 1);
       if (!is_v && w.units) mbar_wait(q_full, (w.units - 1) & 1);
-    } else {   // warp 1: scores of query tile 0; warp 3: of query tile 1
-      const int i = warp == 1 ? 0 : 1;
-      constexpr uint32_t idesc = descriptor(K::format, TQ, TK, false);
-      const uint32_t d = tmem + S_COL + 128 * i;
-      int g = 0, n = 0;   // tiles of the ring and of this chain
-      bool ok = true;
-      for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
-        const Share share(p, w, i, tile_tokens);
-        const uint64_t q = tc::sw128_desc(smem_addr(sq + (share.split ? 0 : i) * C::q_bytes));
-        if (!tc::wait_w(q_full, w.units & 1, abort_flag)) { ok = false; break; }
-        for (int t = 0; t < w.t1 - w.t0; ++t, ++g) {
-          const int s = g % C::stages;
-          ok = tc::wait_w(k_full + s, (g / C::stages) & 1, abort_flag);
-          if (!ok) break;
-          if (!share.mine(i, t)) {
-            if (lane == 0) tc::mbar_arrive(k_empty + s);
-            continue;
-          }
-          // S(n) goes where P(n - 2) was
-          ok = n < 2 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2));
-          if (!ok) break;
-          tc::fence_after();
-          issue_scores<D>(d + 64 * (n & 1), q, tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
-                          s_full + 2 * i + (n & 1), k_empty + s);
-          ++n;
-        }
-        if (!ok) break;
-        if (share.count) tc::commit_w(q_empty);
-        else if (lane == 0) tc::mbar_arrive(q_empty);
-      }
-      tc::commit_w(drained);
+    } else if (warp == 1 || kChains == 2) {   // warp 1: scores of query tile 0; warp 3: of query tile 1
+      issue_all_scores(warp == 1 ? 0 : 1);
+    } else {   // warp 3: O of the query tile
+      issue_all_values(0);
     }
-    // Teardown: the TMEM owner frees the columns once all 14 warps are past their last TMEM access.
+    // Teardown: the TMEM owner frees the columns once all warps are past their last TMEM access.
     tc::fence_before();
     __syncwarp();
     asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
     if (warp == 1) {
       mbar_wait(drained, 0);
       tc::fence_after();
-      tc::tmem_dealloc(*tmem_slot, TMEM_COLS);
+      tc::tmem_dealloc(*tmem_slot, C::tmem_cols);
     }
     return;
   }
 
   if (warp >= 12) {   // warp 12: O of query tile 0; warp 13: of query tile 1
-    const int i = warp - 12;
-    constexpr uint32_t idesc = descriptor(K::format, TQ, D, true);
-    const uint32_t d = tmem + O_COL + 128 * i, a = tmem + S_COL + 128 * i;
-    int g = 0, n = 0;
-    bool ok = true;
-    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
-      const Share share(p, w, i, tile_tokens);
-      bool fresh = true;   // a unit's first product starts O afresh
-      for (int t = 0; t < w.t1 - w.t0; ++t, ++g) {
-        const int s = g % C::stages;
-        ok = tc::wait_w(v_full + s, (g / C::stages) & 1, abort_flag);
-        if (!ok) break;
-        if (!share.mine(i, t)) {
-          if (lane == 0) tc::mbar_arrive(v_empty + s);
-          continue;
-        }
-        ok = __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
-        if (!ok) break;
-        tc::fence_after();
-        issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc, !fresh,
-                     pv_done + 2 * i + (n & 1), v_empty + s);
-        fresh = false;
-        ++n;
-      }
-    }
-    tc::commit_w(drained);
+    issue_all_values(warp - 12);
     tc::fence_before();
     __syncwarp();
     asm volatile("barrier.arrive 1, %0;" ::"n"(kThreads) : "memory");
@@ -462,10 +482,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 
   const int i = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-  const uint32_t to = tmem + lanes + O_COL + 128 * i;
+  const uint32_t to = tmem + lanes + C::o_col + 128 * i;
   const float sl2 = p.scale_log2;
   const bool in_tile = row < tile_tokens * p.group;
-  int n0 = 0, splits = 0;
+  int n0 = 0;
   bool ok = true;
   Walk w(p, place);
   for (; ok && w.more(); w.next(p, place)) {
@@ -473,17 +493,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     if (p.status && threadIdx.x == 128) {
       if (__ldg(p.lengths + at.s) != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
     }
-    const Share share(p, w, i, tile_tokens);
-    const int token = at.j * p.unit_tokens + (share.split ? 0 : i * tile_tokens) + row / p.group;
+    if (idle(w, i)) continue;
+    const int token = at.j * p.unit_tokens + i * tile_tokens + row / p.group;
     const bool live = in_tile && token < at.q.n;
     // Keys that this row sees; a dead row's result is not stored.
     const int limit = !live ? 0 : p.causal ? max(0, min(at.q.len, at.q.len - at.q.n + token + 1)) : at.q.len;
     const int least = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
     const bool warp_live = least != 0x7fffffff;
     float m_used = -INFINITY, l_run = 0.f;
-    for (int u = 0; u < share.count; ++u) {
+    const int count = w.t1 - w.t0;
+    int key0 = w.t0 * TK;
+    for (int u = 0; u < count; ++u, key0 += TK) {
       const int n = n0 + u, buffer = n & 1;
-      const uint32_t ts = tmem + lanes + S_COL + 128 * i + 64 * buffer;
+      const uint32_t ts = tmem + lanes + C::s_col + 128 * i + 64 * buffer;
       if (!buffer_wait(s_full, i, n)) { ok = false; break; }
       if (!warp_live) {
         __syncwarp();
@@ -495,7 +517,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       tc::ld32(ts, r[0]);
       tc::ld32(ts + 32, r[1]);
       tc::wait_ld();
-      const int key0 = (w.t0 + share.tile(i, u)) * TK;
       if (key0 + TK > least) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -541,14 +562,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       if (any_raise && u >= 1) {   // O holds the products of the earlier tiles once P(t - 1) V(t - 1) is done
         if (!buffer_wait(pv_done, i, n - 1)) { ok = false; break; }
         tc::fence_after();
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tc::ld32(to + c * 32, o);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          uint32_t o[16];
+          ld16(to + c, o);
           tc::wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-          tc::st32(to + c * 32, o);
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+          tc::st16(to + c, o);
         }
       }
       tc::wait_st();
@@ -558,128 +579,72 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_full + 2 * i + buffer);
     }
-    if (ok && share.count) ok = buffer_wait(pv_done, i, n0 + share.count - 1);
+    if (ok) ok = buffer_wait(pv_done, i, n0 + count - 1);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     tc::fence_after();
-    n0 += share.count;
+    n0 += count;
     const bool whole = w.t0 == 0 && w.t1 == at.tiles;
     // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
     // makes the row NaN, as inf - inf does.
     if (m_used == INFINITY) l_run = __int_as_float(0x7fffffff);
     if (m_used == -INFINITY) l_run = 0.f;
-    float factor = m_used == -INFINITY ? 0.f : 1.f, other_factor = 0.f;
-    if (share.split && i == 1) {
-      if (splits >= 1) ok = __all_sync(0xffffffffu, tc::wait(split_free, (splits - 1) & 1, abort_flag));
-      if (!ok) break;
-      if (warp_live) {
-        if (live) p.split_ml[(int64_t)cta * TQ + row] = make_float2(m_used, l_run);
-        float4* dst = reinterpret_cast<float4*>(p.split_o) + (int64_t)cta * TQ * (D / 4) + row;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tc::ld32(to + c * 32, o);
-          tc::wait_ld();
-          if (live && factor != 0.f) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              dst[(c * 8 + k) * TQ] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
-                                                  __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
-          }
-        }
-      }
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(split_full);
-      ++splits;
-      continue;
-    }
-    if (share.split) {   // the second chain's sums join the first's
-      ok = __all_sync(0xffffffffu, tc::wait(split_full, splits & 1, abort_flag));
-      if (!ok) break;
-      if (live) {
-        const float2 ml = __ldcg(p.split_ml + (int64_t)cta * TQ + row);
-        const float m_new = max2_nan(m_used, ml.x);
-        other_factor = ml.x == -INFINITY ? 0.f : ml.x == m_new ? 1.f : tc::ex2(ml.x - m_new);
-        factor = m_used == -INFINITY ? 0.f : m_used == m_new ? 1.f : tc::ex2(m_used - m_new);
-        l_run = l_run * factor + ml.y * other_factor;
-        m_used = m_new;
-      }
-    }
     const bool none = m_used == -INFINITY;
-    const float inverse = !whole ? 1.f : none ? 0.f : 1.f / l_run;
+    const float factor = none ? 0.f : whole ? 1.f / l_run : 1.f;
     if (warp_live) {
-      // Columns [c, c + 32) of this thread's row.
-      auto columns = [&](int c, float (&f)[32]) {
-        uint32_t o[32];
-        tc::ld32(to + c, o);
+      const int64_t slot = 2 * cta + (w.part > 0 ? 1 : 0);
+      const int part_row = i * TQ + row;
+      float4* part = reinterpret_cast<float4*>(p.partial_o) + slot * p.rows * (D / 4) + part_row;
+      const int64_t row0 = (int64_t)(at.q.row0 + at.j * p.unit_tokens) * p.q_heads + at.h * p.group;
+      const int out_row = live ? (token - at.j * p.unit_tokens) * p.q_heads + row % p.group : -1;
+      uint8_t* mine = so + (warp - 4) * 32 * C::out_row;
+      // Sixteen columns at a time, in a loop kept small: code that runs once a unit is fetched anew by every SM, and an
+      // unrolled form of this took longer (2.3 us a unit of two 96-wide tiles, 1.6 for its sums).
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t o[16];
+        ld16(to + c, o);
         tc::wait_ld();
+        float f[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = factor == 0.f ? 0.f : __uint_as_float(o[j]) * factor;
-        if (live && other_factor != 0.f) {   // NaN too
-          const float4* src = reinterpret_cast<const float4*>(p.split_o) + (int64_t)cta * TQ * (D / 4) + row;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float4 x = __ldcg(src + (c / 4 + k) * TQ);
-            f[4 * k] = fmaf(x.x, other_factor, f[4 * k]);
-            f[4 * k + 1] = fmaf(x.y, other_factor, f[4 * k + 1]);
-            f[4 * k + 2] = fmaf(x.z, other_factor, f[4 * k + 2]);
-            f[4 * k + 3] = fmaf(x.w, other_factor, f[4 * k + 3]);
-          }
-        }
-      };
-      if (!whole) {   // neighbouring rows are neighbours in memory
-        const int64_t slot = 2 * cta + (w.part > 0 ? 1 : 0);
-        const int r = (share.split ? 0 : i * TQ) + row;
-        float4* dst = reinterpret_cast<float4*>(p.partial_o) + slot * p.rows * (D / 4) + r;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float f[32];
-          columns(c, f);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (live) dst[(c / 4 + k) * p.rows] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
-        }
-        if (live) p.partial_ml[slot * p.rows + r] = make_float2(m_used, l_run);
-      } else {   // through shared memory, so that eight lanes write 128 bytes of a row
-        const int64_t row0 = (int64_t)(at.q.row0 + at.j * p.unit_tokens) * p.q_heads + at.h * p.group;
-        const int out_row = live ? (token - at.j * p.unit_tokens) * p.q_heads + row % p.group : -1;
-        uint8_t* mine = so + (warp - 4) * 4096;
-#pragma unroll
-        for (int c = 0; c < D; c += 64) {
-          constexpr int wide = 64;
-          const int pieces = (D - c < wide ? D - c : wide) / 8;   // of 16 bytes a row
-#pragma unroll
-          for (int b = 0; b < pieces / 4; ++b) {
-            float f[32];
-            columns(c + 32 * b, f);
+        for (int j = 0; j < 16; ++j) f[j] = none ? 0.f : __uint_as_float(o[j]) * factor;
+        if (!whole) {   // neighbouring rows are neighbours in memory
+          if (live) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(mine + lane * 128 + (((4 * b + k) ^ (lane & 7)) * 16)) =
-                  make_uint4(K::pack(f[8 * k] * inverse, f[8 * k + 1] * inverse),
-                             K::pack(f[8 * k + 2] * inverse, f[8 * k + 3] * inverse),
-                             K::pack(f[8 * k + 4] * inverse, f[8 * k + 5] * inverse),
-                             K::pack(f[8 * k + 6] * inverse, f[8 * k + 7] * inverse));
+              part[(c / 4 + k) * p.rows] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
           }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < pieces; ++k) {
-            const int r = (32 * k + lane) / pieces, piece = lane % pieces;
-            const int to_row = __shfl_sync(0xffffffffu, out_row, r);
-            const uint4 x = *reinterpret_cast<const uint4*>(mine + r * 128 + ((piece ^ (r & 7)) * 16));
-            if (to_row >= 0)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + to_row) * D + c + piece * 8) = x;
-          }
-          __syncwarp();
+          continue;
         }
-        if (live && p.lse)
-          p.lse[row0 + out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
+        // Through shared memory, so that the lanes of a row write its 64 or 128 bytes together. Pieces of 16 bytes are
+        // swizzled: by the row for rows of 128 bytes, by every second row for rows of 64.
+        auto place_of = [&](int r, int piece) {
+          return reinterpret_cast<uint4*>(mine + r * C::out_row +
+                                          ((kChains == 2 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3)) * 16));
+        };
+        const int piece0 = c % C::out_cols / 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *place_of(lane, piece0 + k) =
+              make_uint4(K::pack(f[8 * k], f[8 * k + 1]), K::pack(f[8 * k + 2], f[8 * k + 3]),
+                         K::pack(f[8 * k + 4], f[8 * k + 5]), K::pack(f[8 * k + 6], f[8 * k + 7]));
+        if (piece0 + 2 < C::out_cols / 8 && c + 16 < D) continue;
+        __syncwarp();
+        const int shift = piece0 == 6 ? 3 : 2;   // log2 of the row's pieces: 8 or 4
+#pragma unroll 4
+        for (int k = 0; k < 1 << shift; ++k) {
+          const int e = 32 * k + lane, r = e >> shift, piece = e & ((1 << shift) - 1);
+          const int to_row = __shfl_sync(0xffffffffu, out_row, r);
+          const uint4 x = *place_of(r, piece);
+          if (to_row >= 0)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + to_row) * D + c / C::out_cols * C::out_cols +
+                                      piece * 8) = x;
+        }
+        __syncwarp();
       }
-    }
-    if (share.split) {
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(split_free);
-      ++splits;
+      if (live && !whole) p.partial_ml[slot * p.rows + part_row] = make_float2(m_used, l_run);
+      if (live && whole && p.lse)
+        p.lse[row0 + out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
     }
     if (threadIdx.x == 128 && w.part == 0 && !whole && w.t1 == at.tiles)
       p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + at.j * p.unit_tokens,
@@ -736,7 +701,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const Params p) {
   const int out_row = live ? token * p.q_heads + in_tile % join.group : -1;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint4*>(stage[warp] + lane * 64 + ((k ^ (lane & 3)) * 16)) =
+    *reinterpret_cast<uint4*>(stage[warp] + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16)) =
         make_uint4(Kind<T>::pack(f[8 * k] * inverse, f[8 * k + 1] * inverse),
                    Kind<T>::pack(f[8 * k + 2] * inverse, f[8 * k + 3] * inverse),
                    Kind<T>::pack(f[8 * k + 4] * inverse, f[8 * k + 5] * inverse),
@@ -745,26 +710,33 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const Params p) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int q = 8 * k + lane / 4, piece = lane % 4, to_row = __shfl_sync(0xffffffffu, out_row, q);
-    const uint4 x = *reinterpret_cast<const uint4*>(stage[warp] + q * 64 + ((piece ^ (q & 3)) * 16));
+    const uint4 x = *reinterpret_cast<const uint4*>(stage[warp] + q * 64 + ((piece ^ ((q >> 1) & 3)) * 16));
     if (to_row >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + to_row) * D + c + piece * 8) = x;
   }
   if (live && c == 0 && p.lse)
     p.lse[row0 + out_row] = total == 0.f ? -INFINITY : (top - Kind<T>::shift + log2f(total)) * 0.69314718056f;
 }
 
-template <typename T, int D>
+template <typename T, int D, int kChains>
 int launch(const Maps& maps, const Params& p, int ctas, cudaStream_t stream) {
+  using C = Tiles<D, kChains>;
   static PerDevice<int> ready;
   int unused;
-  const int rc = ready.get(&unused, [](int, int*) -> int {
-    SVX_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tiles<D>::smem));
+  int rc = ready.get(&unused, [](int, int*) -> int {
+    SVX_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<T, D, kChains>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem));
     return SVX_OK;
   });
+  if (!rc) rc = launch_dependent("chunk_kernel", chunk_kernel<T, D, kChains>, dim3(ctas), dim3(C::threads), C::smem, stream, maps, p);
   if (rc) return rc;
-  if (const int rc = launch_dependent("chunk_kernel", chunk_kernel<T, D>, dim3(ctas), dim3(kThreads), Tiles<D>::smem,
-                                      stream, maps, p))
-    return rc;
-  return launch_dependent("chunk_join_kernel", chunk_join_kernel<T, D>, dim3(ctas, D / 32), dim3(256), 0, stream, p);
+  return launch_dependent("chunk_join_kernel", chunk_join_kernel<T, D>, dim3(ctas, p.rows / 32 * (D / 32) / 8), dim3(256), 0, stream, p);
+}
+
+template <typename T>
+int launch(const Maps& maps, const Params& p, int dim, int ctas, cudaStream_t stream) {
+  const bool two = p.unit_tokens > p.tile_tokens;
+  if (dim == 64) return two ? launch<T, 64, 2>(maps, p, ctas, stream) : launch<T, 64, 1>(maps, p, ctas, stream);
+  if (dim == 96) return two ? launch<T, 96, 2>(maps, p, ctas, stream) : launch<T, 96, 1>(maps, p, ctas, stream);
+  return two ? launch<T, 128, 2>(maps, p, ctas, stream) : launch<T, 128, 1>(maps, p, ctas, stream);
 }
 
 }  // namespace
@@ -778,14 +750,8 @@ int chunk_launch(const Params& p, int dtype, int dim, int ctas, cudaStream_t str
   if (!rc) rc = make_map_3d(&maps.k, p.k, dim, pools, page, (uint64_t)page * dim * 2, dim * 2, 64, box);
   if (!rc) rc = make_map_3d(&maps.v, p.v, dim, pools, page, (uint64_t)page * dim * 2, dim * 2, 64, box);
   if (rc) return rc;
-  if (dtype == SVX_BF16) {
-    if (dim == 64) return launch<__nv_bfloat16, 64>(maps, p, ctas, stream);
-    if (dim == 96) return launch<__nv_bfloat16, 96>(maps, p, ctas, stream);
-    return launch<__nv_bfloat16, 128>(maps, p, ctas, stream);
-  }
-  if (dim == 64) return launch<__half, 64>(maps, p, ctas, stream);
-  if (dim == 96) return launch<__half, 96>(maps, p, ctas, stream);
-  return launch<__half, 128>(maps, p, ctas, stream);
+  if (dtype == SVX_BF16) return launch<__nv_bfloat16>(maps, p, dim, ctas, stream);
+  return launch<__half>(maps, p, dim, ctas, stream);
 }
 
 }  // namespace paged
