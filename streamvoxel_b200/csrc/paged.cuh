@@ -66,26 +66,19 @@ __device__ __forceinline__ int token_tiles(const Params& p, const Sequence& q) {
   return (q.n + p.unit_tokens - 1) / p.unit_tokens;
 }
 
-// sum of floor((a i + b) / m) over i in [0, n), a, b >= 0: the lattice points under a line, by Euclid's algorithm.
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t sum = 0;
-  while (true) {
-    if (a >= m) {
-      sum += n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
-    }
-    const int64_t y = a * n + b;
-    if (y < m) return sum;
-    n = y / m;
-    b = y % m;
-    const int64_t t = m;
-    m = a;
-    a = t;
-  }
+// x / y, mostly of values below 2^32.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// sum of floor((a i + b) / 64) over i in [0, n), a, b >= 0: of the terms themselves, without their residues mod 64, which
+// repeat every 64 / gcd(a, 64) terms; a whole period holds every residue that is b's mod the gcd once.
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int a, int64_t b) {
+  const int g = (a & 63) ? (a & -a) : 64, period = 64 / g;
+  const int64_t periods = n / period;
+  int64_t residues = periods * ((int64_t)period * (b & (g - 1)) + g * (period * (period - 1) / 2));
+  for (int i = 0; i < (int)(n - periods * period); ++i) residues += ((int64_t)a * i + b) & 63;
+  return (a * (n * (n - 1) / 2) + b * n - residues) >> 6;
 }
 
 // Key tiles of the first `count` token tiles of a sequence, for one head.
@@ -98,7 +91,7 @@ __device__ __forceinline__ int64_t tiles_before(const Params& p, const Sequence&
   const int ones = base >= kTile ? 0 : min(full, (kTile - base) / p.unit_tokens);
   int64_t sum = ones;
   if (full > ones)
-    sum += floor_sum(full - ones, kTile, p.unit_tokens, (int64_t)base + (int64_t)(ones + 1) * p.unit_tokens + kTile - 1);
+    sum += floor_sum(full - ones, p.unit_tokens, (int64_t)base + (int64_t)(ones + 1) * p.unit_tokens + kTile - 1);
   if (count > full) sum += unit_tiles(unit_limit(p, q, full));
   return sum;
 }
@@ -107,32 +100,34 @@ __device__ __forceinline__ int64_t tiles_before(const Params& p, const Sequence&
 struct Place {
   int waves;
   int s, j, h, t;       // where the run begins
+  Sequence q;           // sequence s
   int count;            // its tiles
   int first, first_slot;  // for the join of the unit that the run begins inside of: see Join
 };
 
 struct PlanShared {
-  int64_t warp_tiles[20], warp_units[20];   // of at most 640 threads
+  int64_t warp_tiles[16], warp_units[16];   // of at most 512 threads
   Place place;
 };
 
-// Sums over the block of two values; *before: of the threads before this one.
-template <int kThreads>
+// Sums over the block of one value or (kBoth) two; *before: of the threads before this one.
+template <int kThreads, bool kBoth>
 __device__ __forceinline__ void block_scan(int64_t a, int64_t b, PlanShared& sh, int64_t* before_a, int64_t* before_b,
                                            int64_t* total_a, int64_t* total_b) {
   int64_t sa = a, sb = b;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t oa = __shfl_up_sync(0xffffffffu, sa, d), ob = __shfl_up_sync(0xffffffffu, sb, d);
-    if (lane_id() >= d) {
-      sa += oa;
-      sb += ob;
+    const int64_t oa = __shfl_up_sync(0xffffffffu, sa, d);
+    if (lane_id() >= d) sa += oa;
+    if (kBoth) {
+      const int64_t ob = __shfl_up_sync(0xffffffffu, sb, d);
+      if (lane_id() >= d) sb += ob;
     }
   }
   __syncthreads();
   if (lane_id() == 31) {
     sh.warp_tiles[warp_id()] = sa;
-    sh.warp_units[warp_id()] = sb;
+    if (kBoth) sh.warp_units[warp_id()] = sb;
   }
   __syncthreads();
   *before_a = sa - a;
@@ -140,12 +135,14 @@ __device__ __forceinline__ void block_scan(int64_t a, int64_t b, PlanShared& sh,
   *total_a = *total_b = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp_id()) {
-      *before_a += sh.warp_tiles[w];
-      *before_b += sh.warp_units[w];
+    const int64_t x = sh.warp_tiles[w];
+    *before_a += w < warp_id() ? x : 0;
+    *total_a += x;
+    if (kBoth) {
+      const int64_t y = sh.warp_units[w];
+      *before_b += w < warp_id() ? y : 0;
+      *total_b += y;
     }
-    *total_a += sh.warp_tiles[w];
-    *total_b += sh.warp_units[w];
   }
 }
 
@@ -157,11 +154,16 @@ struct Cursor {
     limit = unit_limit(p, q, j);
     tiles = unit_tiles(limit);
   }
-  __device__ __forceinline__ void set(const Params& p, int s_, int j_, int h_) {
-    s = s_;
-    j = j_;
-    h = h_;
-    q = load_sequence(p, s);
+  __device__ __forceinline__ void set(const Params& p, const Place& place) {
+    s = place.s;
+    j = place.j;
+    h = place.h;
+    q = place.q;
+    see(p);
+  }
+  __device__ __forceinline__ void first(const Params& p) {
+    s = j = h = 0;
+    q = load_sequence(p, 0);
     see(p);
   }
   __device__ __forceinline__ void next(const Params& p) {
@@ -209,15 +211,16 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
   const int per = (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(p.sequences, tid * per), s1 = min(p.sequences, s0 + per);
   int64_t tiles = 0, units = 0;
+  Sequence q{};
   for (int s = s0; s < s1; ++s) {
-    const Sequence q = load_sequence(p, s);
+    q = load_sequence(p, s);
     const int n = token_tiles(p, q);
     tiles += tiles_before(p, q, n) * heads;
-    units += (int64_t)n * heads;
+    if (kWaves) units += (int64_t)n * heads;
   }
   int64_t before, units_before, total, units_total;
-  block_scan<kThreads>(tiles, units, sh, &before, &units_before, &total, &units_total);
-  const int64_t each = max((int64_t)p.min_tiles, (total + ctas - 1) / ctas);
+  block_scan<kThreads, kWaves>(tiles, units, sh, &before, &units_before, &total, &units_total);
+  const int64_t each = max((int64_t)p.min_tiles, quotient(total + ctas - 1, ctas));
   int waves = 0;
   // The last wave and the rest stay for the runs. A step of `ctas` units reads every sequence that it passes, one after the
   // other, so they are not to be many.
@@ -232,7 +235,7 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
       dealt_tiles = 0;
       if (tid < ctas) {
         Cursor u;
-        u.set(p, 0, 0, 0);
+        u.first(p);
         bool ok = u.skip(p, tid);
         for (int k = 0; ok && k < waves; ++k) {
           dealt_tiles += u.tiles;
@@ -248,7 +251,7 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
     }
     const int64_t need = tid < ctas ? each - dealt_tiles : 0;   // waves == 0: equal runs of the whole line
     int64_t need_before, dealt_before, need_total, dealt_total;
-    block_scan<kThreads>(need, dealt_tiles, sh, &need_before, &dealt_before, &need_total, &dealt_total);
+    block_scan<kThreads, true>(need, dealt_tiles, sh, &need_before, &dealt_before, &need_total, &dealt_total);
     if (tid < ctas) scratch[tid] = min(total, dealt_total + need_before);
     if (tid == 0) scratch[ctas] = total;
     __syncthreads();
@@ -262,11 +265,11 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
   if (begin < end && begin >= before && begin < before + tiles) {
     int64_t at = before;
     for (int s = s0; s < s1; ++s) {
-      const Sequence q = load_sequence(p, s);
+      if (per > 1) q = load_sequence(p, s);
       const int n = token_tiles(p, q);
       const int64_t head = tiles_before(p, q, n);
       if (begin < at + head * heads) {
-        const int h = (int)((begin - at) / head);
+        const int h = (int)quotient(begin - at, head);
         at += h * head;
         int lo = 0, hi = n - 1;   // the last token tile that begins at or before the place
         while (lo < hi) {
@@ -275,11 +278,12 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
         }
         at += tiles_before(p, q, lo);
         sh.place.s = s;
+        sh.place.q = q;
         sh.place.j = lo;
         sh.place.h = h;
         sh.place.t = (int)(begin - at);
         // The CTA whose run holds the unit's first tile.
-        int first = (int)(at / each);
+        int first = (int)quotient(at, each);
         if (kWaves && waves) {
           first = 0;
           int top = c;

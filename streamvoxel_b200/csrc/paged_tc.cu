@@ -219,7 +219,7 @@ struct Walk {
     part = -1;
     t0 = t1 = 0;
     if (waves) {
-      at.set(p, 0, 0, 0);
+      at.first(p);
       at.skip(p, blockIdx.x);
       t1 = at.tiles;
     } else {
@@ -229,7 +229,7 @@ struct Walk {
   __device__ __forceinline__ void start_run(const Params& p, const Place& place) {
     if (left <= 0) return;
     part = 0;
-    at.set(p, place.s, place.j, place.h);
+    at.set(p, place);
     t0 = place.t;
     t1 = min(at.tiles, t0 + left);
   }
@@ -673,26 +673,30 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const Params p) {
   const int warp = warp_id(), lane = lane_id(), task = blockIdx.y * 8 + warp;
   const int r = task / (D / 32) * 32 + lane, c = task % (D / 32) * 32, in_tile = r % p.tile_rows;
   const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
-  const bool live = in_tile < p.tile_tokens * join.group && token < join.tokens;
+  const bool live = r < p.rows && in_tile < p.tile_tokens * join.group && token < join.tokens;
   if (!__any_sync(0xffffffffu, live)) return;
   auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)); };
   float top = -INFINITY, total = 0.f, f[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[j] = 0.f;
   if (live) {
-    for (int i = 0; i < join.parts; ++i) top = fmaxf(top, p.partial_ml[slot(i) * p.rows + r].x);
-    for (int i = 0; i < join.parts; ++i) {
+    const float4* src = reinterpret_cast<const float4*>(p.partial_o) + c / 4 * p.rows + r;
+#pragma unroll 2
+    for (int i = 0; i < join.parts; ++i) {   // the loads of two parts are on their way together
       const float2 ml = p.partial_ml[slot(i) * p.rows + r];
-      const float4* src = reinterpret_cast<const float4*>(p.partial_o) + slot(i) * p.rows * (D / 4) + c / 4 * p.rows + r;
-      const float x = ml.x == top ? 1.f : tc::ex2(ml.x - top);
-      total = fmaf(ml.y, x, total);
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = src[slot(i) * p.rows * (D / 4) + k * p.rows];
+      const float now = fmaxf(top, ml.x);
+      const float old = top == now ? 1.f : tc::ex2(top - now), x = ml.x == now ? 1.f : tc::ex2(ml.x - now);
+      top = now;
+      total = fmaf(ml.y, x, total * old);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float4 v = src[k * p.rows];
-        f[4 * k] = fmaf(v.x, x, f[4 * k]);
-        f[4 * k + 1] = fmaf(v.y, x, f[4 * k + 1]);
-        f[4 * k + 2] = fmaf(v.z, x, f[4 * k + 2]);
-        f[4 * k + 3] = fmaf(v.w, x, f[4 * k + 3]);
+        f[4 * k] = fmaf(v[k].x, x, f[4 * k] * old);
+        f[4 * k + 1] = fmaf(v[k].y, x, f[4 * k + 1] * old);
+        f[4 * k + 2] = fmaf(v[k].z, x, f[4 * k + 2] * old);
+        f[4 * k + 3] = fmaf(v[k].w, x, f[4 * k + 3] * old);
       }
     }
   }
@@ -728,7 +732,7 @@ int launch(const Maps& maps, const Params& p, int ctas, cudaStream_t stream) {
   });
   if (!rc) rc = launch_dependent("chunk_kernel", chunk_kernel<T, D, kChains>, dim3(ctas), dim3(C::threads), C::smem, stream, maps, p);
   if (rc) return rc;
-  return launch_dependent("chunk_join_kernel", chunk_join_kernel<T, D>, dim3(ctas, p.rows / 32 * (D / 32) / 8), dim3(256), 0, stream, p);
+  return launch_dependent("chunk_join_kernel", chunk_join_kernel<T, D>, dim3(ctas, (p.rows / 32 * (D / 32) + 7) / 8), dim3(256), 0, stream, p);
 }
 
 template <typename T>

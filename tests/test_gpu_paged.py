@@ -281,7 +281,7 @@ def test_attention_hint_changes_nothing(ops, hint, news):
 
 
 @pytest.mark.parametrize('heads,group,dim,news', [(1, 1, 64, 1), (1, 8, 128, 1), (2, 4, 128, 3), (1, 1, 96, 40),
-                                                  (1, 4, 128, 300)])
+                                                  (1, 4, 128, 300), (1, 4, 96, 20), (1, 2, 96, 300)])
 def test_attention_one_long_sequence(ops, heads, group, dim, news):
     """The keys of one sequence are divided over the whole card and joined."""
     rng, g = np.random.default_rng(3), torch.Generator().manual_seed(3)

@@ -166,15 +166,13 @@ def _line(lengths, news, heads, unit_tokens, causal):
 def test_closed_form_of_the_tile_count():
     """The kernels find their place on the line of tiles by a closed form (a floor sum): the same, restated, against
     counting."""
-    def floor_sum(n, m, a, b):
-        total = 0
-        while True:
-            total += n * (n - 1) // 2 * (a // m) + n * (b // m)
-            a, b = a % m, b % m
-            y = a * n + b
-            if y < m:
-                return total
-            n, b, m, a = y // m, y % m, a, m
+    def floor_sum(n, a, b):
+        g = a & -a if a % 64 else 64
+        period = 64 // g
+        periods = n // period
+        residues = periods * (period * (b % g) + g * period * (period - 1) // 2)
+        residues += sum((a * i + b) % 64 for i in range(n - periods * period))
+        return (a * (n * (n - 1) // 2) + b * n - residues) // 64
 
     def tiles_before(length, n, unit, causal, count):
         if not count:
@@ -189,7 +187,7 @@ def test_closed_form_of_the_tile_count():
         ones = 0 if base >= 64 else min(full, (64 - base) // unit)
         total = ones
         if full > ones:
-            total += floor_sum(full - ones, 64, unit, base + (ones + 1) * unit + 63)
+            total += floor_sum(full - ones, unit, base + (ones + 1) * unit + 63)
         return total + (one(seen(full)) if count > full else 0)
 
     rng = np.random.default_rng(0)
