@@ -378,9 +378,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   float top = -INFINITY, total = 0.f;
   if (live) {
     for (int i0 = share; i0 < join.parts; i0 += 32 * kWarpsRow) {
-      const int i = i0 + kWarpsRow * lane;   // this warp's parts
+      const int i = i0 + kWarpsRow * lane, here = min(32, (join.parts - i0 + kWarpsRow - 1) / kWarpsRow);   // this warp's parts
       float2 ml = make_float2(-INFINITY, 0.f);
       if (i < join.parts) ml = p.partial_ml[slot(i)];
+      // Eight parts' columns are on their way at a time, the first of them with the bases.
+      float4 v[8];
+      auto load = [&](int x0) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (x0 + x < here && lane < D / 4)
+            v[x] = *reinterpret_cast<const float4*>(p.partial_o + slot(i0 + kWarpsRow * (x0 + x)) * D + 4 * lane);
+      };
+      load(0);
       float now = ml.x;
 #pragma unroll
       for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
@@ -393,15 +402,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
       total = total * old + add;
       sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
       top = now;
-      const int here = min(32, (join.parts - i0 + kWarpsRow - 1) / kWarpsRow);
-#pragma unroll 4
-      for (int x = 0; x < here; ++x) {
-        const float fx = __shfl_sync(0xffffffffu, f, x);
-        if (lane < D / 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.partial_o + slot(i0 + kWarpsRow * x) * D + 4 * lane);
-          sum.x = fmaf(v.x, fx, sum.x); sum.y = fmaf(v.y, fx, sum.y);
-          sum.z = fmaf(v.z, fx, sum.z); sum.w = fmaf(v.w, fx, sum.w);
+      for (int x0 = 0;;) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float fx = __shfl_sync(0xffffffffu, f, (x0 + x) & 31);
+          if (x0 + x < here && lane < D / 4) {
+            sum.x = fmaf(v[x].x, fx, sum.x); sum.y = fmaf(v[x].y, fx, sum.y);
+            sum.z = fmaf(v[x].z, fx, sum.z); sum.w = fmaf(v[x].w, fx, sum.w);
+          }
         }
+        x0 += 8;
+        if (x0 >= here) break;
+        load(x0);
       }
     }
   }

@@ -110,20 +110,21 @@ struct PlanShared {
   Place place;
 };
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int64_t warp_scan(int64_t x) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane_id() >= d) x += o;
+  }
+  return x;
+}
+
 // Sums over the block of one value or (kBoth) two; *before: of the threads before this one.
 template <int kThreads, bool kBoth>
 __device__ __forceinline__ void block_scan(int64_t a, int64_t b, PlanShared& sh, int64_t* before_a, int64_t* before_b,
                                            int64_t* total_a, int64_t* total_b) {
-  int64_t sa = a, sb = b;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t oa = __shfl_up_sync(0xffffffffu, sa, d);
-    if (lane_id() >= d) sa += oa;
-    if (kBoth) {
-      const int64_t ob = __shfl_up_sync(0xffffffffu, sb, d);
-      if (lane_id() >= d) sb += ob;
-    }
-  }
+  const int64_t sa = warp_scan(a), sb = kBoth ? warp_scan(b) : 0;
   __syncthreads();
   if (lane_id() == 31) {
     sh.warp_tiles[warp_id()] = sa;
@@ -208,8 +209,10 @@ struct Cursor {
 template <int kThreads, bool kWaves>
 __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShared& sh, int64_t* scratch) {
   const int heads = p.kv_heads * p.blocks, tid = threadIdx.x;
-  const int per = (p.sequences + kThreads - 1) / kThreads;
-  const int s0 = min(p.sequences, tid * per), s1 = min(p.sequences, s0 + per);
+  // Up to 32 sequences: every warp adds them up for itself, a lane each, without the block's barriers.
+  const bool few = p.sequences <= 32;
+  const int id = few ? lane_id() : tid, per = few ? 1 : (p.sequences + kThreads - 1) / kThreads;
+  const int s0 = min(p.sequences, id * per), s1 = min(p.sequences, s0 + per);
   int64_t tiles = 0, units = 0;
   Sequence q{};
   for (int s = s0; s < s1; ++s) {
@@ -219,7 +222,15 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
     if (kWaves) units += (int64_t)n * heads;
   }
   int64_t before, units_before, total, units_total;
-  block_scan<kThreads, kWaves>(tiles, units, sh, &before, &units_before, &total, &units_total);
+  if (few) {
+    before = warp_scan(tiles);
+    units_before = kWaves ? warp_scan(units) : 0;
+    total = __shfl_sync(0xffffffffu, before, 31);
+    units_total = __shfl_sync(0xffffffffu, units_before, 31);
+    before -= tiles;
+  } else {
+    block_scan<kThreads, kWaves>(tiles, units, sh, &before, &units_before, &total, &units_total);
+  }
   const int64_t each = max((int64_t)p.min_tiles, quotient(total + ctas - 1, ctas));
   int waves = 0;
   // The last wave and the rest stay for the runs. A step of `ctas` units reads every sequence that it passes, one after the
@@ -262,7 +273,7 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
     sh.place.waves = waves;
     sh.place.count = (int)(end - begin);
   }
-  if (begin < end && begin >= before && begin < before + tiles) {
+  if (begin < end && begin >= before && begin < before + tiles && (!few || tid < 32)) {
     int64_t at = before;
     for (int s = s0; s < s1; ++s) {
       if (per > 1) q = load_sequence(p, s);
