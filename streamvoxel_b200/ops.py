@@ -347,7 +347,10 @@ _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', _raw_stream)
 def _index_of(first, *others):
     """The one CUDA device of the tensors (None entries apart)."""
     index = first.get_device()
-    if index < 0 or any(t is not None and t.get_device() != index for t in others):
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
         raise ValueError('operands must be on one CUDA device')
     return index
 
@@ -498,8 +501,9 @@ def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError('the paged cache takes no part in autograd: call under torch.no_grad()')
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError('the paged cache takes no part in autograd: call under torch.no_grad()')
 
 
 def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=None, positions=None,
@@ -587,7 +591,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
     _no_grad(q, k_pages, v_pages)
     index = _index_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
     if out is None:
-        out = q.new_empty((tokens, heads, dim))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _rows('out', out, tokens, heads, dim, q.dtype)
         if not out.is_contiguous():
@@ -595,7 +599,12 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
     if lse is not None and (lse.shape != (tokens, heads) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise ValueError(f'lse must be a contiguous float32 [{tokens}, {heads}] tensor')
     lib, max_query = _lib.load(), min(int(max_query), tokens)
-    size = lib.svx_paged_attention_workspace_bytes(tokens, cache.sequences, heads, kv_heads, dim, max_query)
+    sizes = tokens, cache.sequences, heads, kv_heads, dim, max_query
+    if index == torch.cuda.current_device():
+        size = lib.svx_paged_attention_workspace_bytes(*sizes)
+    else:
+        with torch.cuda.device(index):
+            size = lib.svx_paged_attention_workspace_bytes(*sizes)
     if workspace is None:
         workspace = q.new_empty((size,), dtype=torch.uint8)
     elif workspace.dtype != torch.uint8 or workspace.numel() < size or not workspace.is_contiguous():
