@@ -18,7 +18,7 @@
 //
 // Measured on B200 (bf16 unless said): 128 sequences of 40 to 16,384 keys, 8 kv heads of 128, 4 query heads each, pages of
 // 16: 278 us, 5.7 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 213 us, 6.1 TB/s; one of 4001
-// keys, 8 heads of 128: 11.4 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
+// keys, 8 heads of 128: 11.5 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
 // joining kernel with the gap before it.
 #include <math.h>
 
@@ -479,14 +479,17 @@ int divide(int tokens, int sequences, int group, int dim, int max_query, bool ch
   if (const int rc = sm_count(&sms)) return rc;
   // Rows for each key: of the longest chunk where the caller knows it, else of the mean one.
   const int64_t query = max_query > 0 ? std::min(max_query, tokens) : (tokens + sequences - 1) / std::max(sequences, 1);
+  // With 17 to 32 rows the few-rows form reads the keys twice: 92 us against 60 for 32 sequences of 300 to 12,000 keys, 4 kv
+  // heads of 128; 17 against 21 for two such sequences, where latency counts.
   d->chunk = chunk_fits && query * group > kRows && group <= 128;
   if (d->chunk) {
     d->group_part = group;
     d->blocks = 1;
     d->tile_tokens = 128 / group;
     // Query tiles of a unit, and then one or two CTAs a SM. Two share the keys' way to the SM (16 chunks of 512 tokens x 4
-    // heads of 128 over 4000 keys: 529 us against 643); one wastes less on chunks that fit a tile, and where the longest
-    // chunk is far above the mean, most do (1 to 700 tokens x 6 heads of 64: 99 us against 110).
+    // heads of 128 over 4000 keys: 530 us against 673); one wastes less on chunks that fit a tile (32 of 5
+    // tokens x 8 heads of 128: 62 us against 83), and where the longest chunk is far above the mean, most do (1 to 700
+    // tokens x 6 heads of 64: 90 us against 99).
     const int64_t mean = tokens / std::max(sequences, 1);
     const bool skewed = max_query > 0 && 4 * mean <= query && mean <= 8 * d->tile_tokens;
     const int tiles = query > d->tile_tokens && !skewed ? 2 : 1;
