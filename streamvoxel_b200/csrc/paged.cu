@@ -6,7 +6,7 @@
 // One pass over the keys with a running maximum m and sum l per row; o, m and l stay in fp32 registers:
 //   m' = max(m, max s), o = o 2^(m - m') + p v, l = l 2^(m - m') + sum p, p = 2^(s - m')
 // (s in log2 units). The weights p are rounded to the cache's type for the product with v, while l sums them
-// unrounded: the rounding of each weight (2^-9 bf16, 2^-12 fp16) is random and averages out over keys, and a row with
+// unrounded: the rounding of each weight (at most 2^-8 bf16, 2^-11 fp16) is random and averages out over keys, and a row with
 // one dominant key has p = 1 there, which is exact. For fp16, whose least step is 2^-24, weights are held 2^7 larger.
 //
 // Bound: the keys and values are read once for the whole group of query heads that share them, so a step with few rows
@@ -17,7 +17,7 @@
 // stages, so the loop has no block barrier; the warps' parts of a unit are merged through shared memory at its end.
 //
 // Measured on B200 (bf16 unless said): 128 sequences of 40 to 16,384 keys, 8 kv heads of 128, 4 query heads each, pages of
-// 16: 278 us, 5.7 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 213 us, 6.1 TB/s; one of 4001
+// 16: 279 us, 5.6 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 213 us, 6.1 TB/s; one of 4001
 // keys, 8 heads of 128: 11.5 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
 // joining kernel with the gap before it.
 #include <math.h>
