@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kern
 
     // The unit's end, or the run's: merge the warps' parts, with the next unit's queries on their way.
     const bool whole = (segment || place.t == 0) && t == at.tiles;
-    const bool ends_first = segment == 0 && !whole && t == at.tiles;
-    const int slot = 2 * cta + (segment ? 1 : 0);
+    const bool ends_others = ends_for_others(segment, whole, t == at.tiles);
+    const int64_t slot = partial_slot(cta, segment);
     const int g0 = at.h % p.blocks * p.group_part, part = min(p.group_part, p.group - g0);
     const int token0 = at.j * p.unit_tokens, tokens = min(p.unit_tokens, at.q.n - token0);
     const int row0 = at.q.row0 + token0, head0 = at.h / p.blocks * p.group + g0;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kern
         sum.z = fmaf(v.z, f[x], sum.z); sum.w = fmaf(v.w, f[x], sum.w);
       }
       if (!whole) {
-        *reinterpret_cast<float4*>(p.partial_o + ((int64_t)slot * p.rows + r) * D + k * 32 + c) = sum;
+        *reinterpret_cast<float4*>(p.partial_o + (slot * p.rows + r) * D + k * 32 + c) = sum;
       } else if (live) {
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + out_row * D + k * 32 + c) =
             make_uint2(Half<T>::pack(sum.x * inverse, sum.y * inverse), Half<T>::pack(sum.z * inverse, sum.w * inverse));
@@ -353,12 +353,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kern
     __syncthreads();
     if (threadIdx.x % 8 == 0) {
       if (!whole) {
-        p.partial_ml[(int64_t)slot * p.rows + r] = make_float2(top_r, sum_r);
+        p.partial_ml[slot * p.rows + r] = make_float2(top_r, sum_r);
       } else if (live && p.lse) {
         p.lse[out_row] = sum_r == 0.f ? -INFINITY : (top_r - Half<T>::shift + log2f(sum_r)) * 0.69314718056f;
       }
     }
-    if (threadIdx.x == 0 && ends_first)
+    if (threadIdx.x == 0 && ends_others)
       p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, row0, tokens, head0, part, 0};
     ++segment;
     t = 0;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const int warp = warp_id(), lane = lane_id(), share = warp % kWarpsRow;
   const int r = blockIdx.y * rows + warp / kWarpsRow, token = r / join.group;
   const bool live = token < join.tokens;
-  auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)) * p.rows + r; };
+  auto slot = [&](int i) { return join.slot(i) * p.rows + r; };
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float top = -INFINITY, total = 0.f;
   if (live) {

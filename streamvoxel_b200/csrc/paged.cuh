@@ -44,36 +44,47 @@ struct Params {
 // second kernel, always in the same order. Calls with several units for each CTA first deal whole units out in waves (CTA
 // c takes units c, c + ctas, ...): the token tiles of one head then run side by side over the same keys, which come from
 // memory once, and only the last units' tiles are divided into runs, whose lengths make every CTA's total equal.
+// All arithmetic of the division is host code too, which the tests run.
+#define SVX_HOST_DEVICE __host__ __device__ __forceinline__
+
+SVX_HOST_DEVICE int32_t entry(const int32_t* at) {
+#ifdef __CUDA_ARCH__
+  return __ldg(at);
+#else
+  return *at;
+#endif
+}
+
 struct Sequence {
   int row0, n, len;   // first row, new tokens, keys
 };
 
-__device__ __forceinline__ Sequence load_sequence(const Params& p, int s) {
+SVX_HOST_DEVICE Sequence load_sequence(const Params& p, int s) {
   Sequence q;
-  q.row0 = max(0, min(__ldg(p.offsets + s), p.tokens));
-  q.n = max(0, min(__ldg(p.offsets + s + 1), p.tokens) - q.row0);
-  q.len = max(0, min(__ldg(p.lengths + s), p.table_width << p.page_shift));
+  q.row0 = max(0, min(entry(p.offsets + s), p.tokens));
+  q.n = max(0, min(entry(p.offsets + s + 1), p.tokens) - q.row0);
+  q.len = max(0, min(entry(p.lengths + s), p.table_width << p.page_shift));
   return q;
 }
 
 // Keys that the last token of token tile j sees.
-__device__ __forceinline__ int unit_limit(const Params& p, const Sequence& q, int j) {
+SVX_HOST_DEVICE int unit_limit(const Params& p, const Sequence& q, int j) {
   if (!p.causal) return q.len;
   return max(0, min(q.len, q.len - q.n + min((j + 1) * p.unit_tokens, q.n)));
 }
-__device__ __forceinline__ int unit_tiles(int limit) { return max(1, (limit + kTile - 1) / kTile); }
-__device__ __forceinline__ int token_tiles(const Params& p, const Sequence& q) {
+SVX_HOST_DEVICE int unit_tiles(int limit) { return max(1, (limit + kTile - 1) / kTile); }
+SVX_HOST_DEVICE int token_tiles(const Params& p, const Sequence& q) {
   return (q.n + p.unit_tokens - 1) / p.unit_tokens;
 }
 
 // x / y, mostly of values below 2^32.
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+SVX_HOST_DEVICE int64_t quotient(int64_t x, int64_t y) {
   return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
 }
 
 // sum of floor((a i + b) / 64) over i in [0, n), a, b >= 0: of the terms themselves, without their residues mod 64, which
 // repeat every 64 / gcd(a, 64) terms; a whole period holds every residue that is b's mod the gcd once.
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int a, int64_t b) {
+SVX_HOST_DEVICE int64_t floor_sum(int64_t n, int a, int64_t b) {
   const int g = (a & 63) ? (a & -a) : 64, period = 64 / g;
   const int64_t periods = n / period;
   int64_t residues = periods * ((int64_t)period * (b & (g - 1)) + g * (period * (period - 1) / 2));
@@ -82,7 +93,7 @@ __device__ __forceinline__ int64_t floor_sum(int64_t n, int a, int64_t b) {
 }
 
 // Key tiles of the first `count` token tiles of a sequence, for one head.
-__device__ __forceinline__ int64_t tiles_before(const Params& p, const Sequence& q, int count) {
+SVX_HOST_DEVICE int64_t tiles_before(const Params& p, const Sequence& q, int count) {
   if (!count) return 0;
   if (!p.causal) return (int64_t)count * unit_tiles(q.len);
   if (count == 1) return unit_tiles(unit_limit(p, q, 0));
@@ -151,23 +162,23 @@ __device__ __forceinline__ void block_scan(int64_t a, int64_t b, PlanShared& sh,
 struct Cursor {
   int s, j, h, limit, tiles;
   Sequence q;
-  __device__ __forceinline__ void see(const Params& p) {
+  SVX_HOST_DEVICE void see(const Params& p) {
     limit = unit_limit(p, q, j);
     tiles = unit_tiles(limit);
   }
-  __device__ __forceinline__ void set(const Params& p, const Place& place) {
+  SVX_HOST_DEVICE void set(const Params& p, const Place& place) {
     s = place.s;
     j = place.j;
     h = place.h;
     q = place.q;
     see(p);
   }
-  __device__ __forceinline__ void first(const Params& p) {
+  SVX_HOST_DEVICE void first(const Params& p) {
     s = j = h = 0;
     q = load_sequence(p, 0);
     see(p);
   }
-  __device__ __forceinline__ void next(const Params& p) {
+  SVX_HOST_DEVICE void next(const Params& p) {
     if (++j >= token_tiles(p, q)) {
       j = 0;
       if (++h >= p.kv_heads * p.blocks) {
@@ -184,7 +195,7 @@ struct Cursor {
     see(p);
   }
   // On by `count` units; false past the last one.
-  __device__ __forceinline__ bool skip(const Params& p, int64_t count) {
+  SVX_HOST_DEVICE bool skip(const Params& p, int64_t count) {
     const int heads = p.kv_heads * p.blocks;
     int per_head = token_tiles(p, q);
     int64_t at = (int64_t)h * per_head + j + count;
@@ -204,24 +215,96 @@ struct Cursor {
   }
 };
 
+// Tiles and units of the sequences [s0, s1), all heads.
+SVX_HOST_DEVICE void add_sequences(const Params& p, int s0, int s1, int64_t* tiles, int64_t* units) {
+  const int heads = p.kv_heads * p.blocks;
+  *tiles = *units = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Sequence q = load_sequence(p, s);
+    const int n = token_tiles(p, q);
+    *tiles += tiles_before(p, q, n) * heads;
+    *units += (int64_t)n * heads;
+  }
+}
+
+// Tiles of a CTA: an equal part of the line.
+SVX_HOST_DEVICE int64_t equal_share(const Params& p, int64_t total, int ctas) {
+  return max((int64_t)p.min_tiles, quotient(total + ctas - 1, ctas));
+}
+
+// Waves of whole units to begin with. The last wave and the rest stay for the runs. A step of `ctas` units reads every
+// sequence that it passes, one after the other, so they are not to be many.
+SVX_HOST_DEVICE int most_waves(const Params& p, int64_t units_total, int ctas) {
+  if (units_total < 2 * (int64_t)ctas || units_total < 64 * (int64_t)p.sequences) return 0;
+  return (int)min(units_total / ctas - 1, (int64_t)1 << 20);
+}
+
+// Tiles of the units that CTA `c` takes whole.
+SVX_HOST_DEVICE int64_t dealt_whole(const Params& p, int c, int ctas, int waves) {
+  int64_t tiles = 0;
+  Cursor u;
+  u.first(p);
+  bool ok = u.skip(p, c);
+  for (int k = 0; ok && k < waves; ++k) {
+    tiles += u.tiles;
+    if (k + 1 < waves) ok = u.skip(p, ctas);
+  }
+  return tiles;
+}
+
+// Where CTA c's run begins: tile `begin` of the line, which lies among the sequences [s0, s1); `before` tiles come before
+// them. line: the runs' begins where units are dealt out whole, null where every run is `each` tiles long.
+SVX_HOST_DEVICE void find_place(const Params& p, int s0, int s1, int64_t before, int64_t begin, int64_t each, int c,
+                                const int64_t* line, Place* place) {
+  const int heads = p.kv_heads * p.blocks;
+  int64_t at = before;
+  for (int s = s0; s < s1; ++s) {
+    const Sequence q = load_sequence(p, s);
+    const int n = token_tiles(p, q);
+    const int64_t head = tiles_before(p, q, n);
+    if (begin < at + head * heads) {
+      const int h = (int)quotient(begin - at, head);
+      at += h * head;
+      int lo = 0, hi = n - 1;   // the last token tile that begins at or before the place
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at + tiles_before(p, q, mid) <= begin) lo = mid; else hi = mid - 1;
+      }
+      at += tiles_before(p, q, lo);
+      place->s = s;
+      place->q = q;
+      place->j = lo;
+      place->h = h;
+      place->t = (int)(begin - at);
+      // The CTA whose run holds the unit's first tile.
+      int first = (int)quotient(at, each);
+      if (line) {
+        first = 0;
+        int top = c;
+        while (first < top) {
+          const int mid = (first + top + 1) >> 1;
+          if (line[mid] <= at) first = mid; else top = mid - 1;
+        }
+      }
+      place->first = first;
+      place->first_slot = at == (line ? line[first] : first * each) ? 0 : 1;
+      return;
+    }
+    at += head * heads;
+  }
+}
+
 // Fills sh.place for CTA `c` of `ctas`; all threads of the block call it. kWaves: deal whole units out first where there
 // are enough of them; `scratch` then holds 8 * ctas + 8 bytes of shared memory.
 template <int kThreads, bool kWaves>
 __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShared& sh, int64_t* scratch) {
-  const int heads = p.kv_heads * p.blocks, tid = threadIdx.x;
+  const int tid = threadIdx.x;
   // Up to 32 sequences: every warp adds them up for itself, a lane each, without the block's barriers.
   const bool few = p.sequences <= 32;
   const int id = few ? lane_id() : tid, per = few ? 1 : (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(p.sequences, id * per), s1 = min(p.sequences, s0 + per);
-  int64_t tiles = 0, units = 0;
-  Sequence q{};
-  for (int s = s0; s < s1; ++s) {
-    q = load_sequence(p, s);
-    const int n = token_tiles(p, q);
-    tiles += tiles_before(p, q, n) * heads;
-    if (kWaves) units += (int64_t)n * heads;
-  }
-  int64_t before, units_before, total, units_total;
+  int64_t tiles, units, before, units_before, total, units_total;
+  add_sequences(p, s0, s1, &tiles, &units);
   if (few) {
     before = warp_scan(tiles);
     units_before = kWaves ? warp_scan(units) : 0;
@@ -231,38 +314,21 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
   } else {
     block_scan<kThreads, kWaves>(tiles, units, sh, &before, &units_before, &total, &units_total);
   }
-  const int64_t each = max((int64_t)p.min_tiles, quotient(total + ctas - 1, ctas));
-  int waves = 0;
-  // The last wave and the rest stay for the runs. A step of `ctas` units reads every sequence that it passes, one after the
-  // other, so they are not to be many.
-  if (kWaves && units_total >= 2 * (int64_t)ctas && units_total >= 64 * (int64_t)p.sequences)
-    waves = (int)min(units_total / ctas - 1, (int64_t)1 << 20);
+  const int64_t each = equal_share(p, total, ctas);
+  int waves = kWaves ? most_waves(p, units_total, ctas) : 0;
   int64_t begin = min(total, each * c), end = min(total, begin + each);
   if (kWaves && waves) {
     // Tiles of the units that each CTA takes whole, which are not to be more than its share; then the runs that fill them
     // up to it.
-    int64_t dealt_tiles = 0;
+    int64_t dealt;
     while (true) {
-      dealt_tiles = 0;
-      if (tid < ctas) {
-        Cursor u;
-        u.first(p);
-        bool ok = u.skip(p, tid);
-        for (int k = 0; ok && k < waves; ++k) {
-          dealt_tiles += u.tiles;
-          if (k + 1 < waves) ok = u.skip(p, ctas);
-        }
-      }
-      if (!__syncthreads_or(dealt_tiles > each)) break;
+      dealt = waves && tid < ctas ? dealt_whole(p, tid, ctas, waves) : 0;
+      if (!__syncthreads_or(dealt > each)) break;
       waves >>= 1;
-      if (!waves) {
-        dealt_tiles = 0;
-        break;
-      }
     }
-    const int64_t need = tid < ctas ? each - dealt_tiles : 0;   // waves == 0: equal runs of the whole line
+    const int64_t need = tid < ctas ? each - dealt : 0;   // waves == 0: equal runs of the whole line
     int64_t need_before, dealt_before, need_total, dealt_total;
-    block_scan<kThreads, true>(need, dealt_tiles, sh, &need_before, &dealt_before, &need_total, &dealt_total);
+    block_scan<kThreads, true>(need, dealt, sh, &need_before, &dealt_before, &need_total, &dealt_total);
     if (tid < ctas) scratch[tid] = min(total, dealt_total + need_before);
     if (tid == 0) scratch[ctas] = total;
     __syncthreads();
@@ -273,45 +339,58 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
     sh.place.waves = waves;
     sh.place.count = (int)(end - begin);
   }
-  if (begin < end && begin >= before && begin < before + tiles && (!few || tid < 32)) {
-    int64_t at = before;
-    for (int s = s0; s < s1; ++s) {
-      if (per > 1) q = load_sequence(p, s);
-      const int n = token_tiles(p, q);
-      const int64_t head = tiles_before(p, q, n);
-      if (begin < at + head * heads) {
-        const int h = (int)quotient(begin - at, head);
-        at += h * head;
-        int lo = 0, hi = n - 1;   // the last token tile that begins at or before the place
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (at + tiles_before(p, q, mid) <= begin) lo = mid; else hi = mid - 1;
-        }
-        at += tiles_before(p, q, lo);
-        sh.place.s = s;
-        sh.place.q = q;
-        sh.place.j = lo;
-        sh.place.h = h;
-        sh.place.t = (int)(begin - at);
-        // The CTA whose run holds the unit's first tile.
-        int first = (int)quotient(at, each);
-        if (kWaves && waves) {
-          first = 0;
-          int top = c;
-          while (first < top) {
-            const int mid = (first + top + 1) >> 1;
-            if (scratch[mid] <= at) first = mid; else top = mid - 1;
-          }
-        }
-        sh.place.first = first;
-        sh.place.first_slot = at == (kWaves && waves ? scratch[first] : first * each) ? 0 : 1;
-        break;
-      }
-      at += head * heads;
-    }
-  }
+  if (begin < end && begin >= before && begin < before + tiles && (!few || tid < 32))
+    find_place(p, s0, s1, before, begin, each, c, kWaves && waves ? scratch : nullptr, &sh.place);
   __syncthreads();
 }
+
+// A CTA's share, unit by unit: key tiles [t0, t1) of the unit at `at`; `part` counts the units of its run of the line (-1:
+// a unit dealt out whole).
+struct Walk {
+  Cursor at;
+  int t0, t1, waves, left, units, part;
+  SVX_HOST_DEVICE Walk(const Params& p, const Place& place, int cta) {
+    waves = place.waves;
+    left = place.count;
+    units = 0;
+    part = -1;
+    t0 = t1 = 0;
+    if (waves) {
+      at.first(p);
+      at.skip(p, cta);
+      t1 = at.tiles;
+    } else {
+      start_run(p, place);
+    }
+  }
+  SVX_HOST_DEVICE void start_run(const Params& p, const Place& place) {
+    if (left <= 0) return;
+    part = 0;
+    at.set(p, place);
+    t0 = place.t;
+    t1 = min(at.tiles, t0 + left);
+  }
+  SVX_HOST_DEVICE bool more() const { return waves > 0 || left > 0; }
+  SVX_HOST_DEVICE bool whole() const { return t0 == 0 && t1 == at.tiles; }
+  SVX_HOST_DEVICE void next(const Params& p, const Place& place, int ctas) {
+    ++units;
+    if (waves) {
+      if (--waves) {
+        at.skip(p, ctas);
+        t1 = at.tiles;
+      } else {
+        start_run(p, place);
+      }
+      return;
+    }
+    left -= t1 - t0;
+    if (left <= 0) return;
+    ++part;
+    at.next(p);
+    t0 = 0;
+    t1 = min(at.tiles, left);
+  }
+};
 
 // Left by CTA c for the joining kernel, where its run ends a unit that an earlier CTA began: the unit's rows and heads,
 // the CTA that began it, and whether the unit was that CTA's first of the line (partial slot 2 first) or its last
@@ -322,7 +401,13 @@ struct Join {
   int row, tokens;         // its tokens' first row, and their count
   int head, group;         // its first query head, and their count
   int pad;
+  // The partial that holds part i.
+  SVX_HOST_DEVICE int64_t slot(int i) const { return 2 * (int64_t)(first + i) + (i == 0 ? first_slot : 0); }
 };
+
+// The partial that CTA c leaves of the unit that is number `part` of its run; whether it ends that unit for others.
+SVX_HOST_DEVICE int64_t partial_slot(int c, int part) { return 2 * (int64_t)c + (part > 0 ? 1 : 0); }
+SVX_HOST_DEVICE bool ends_for_others(int part, bool whole, bool at_end) { return part == 0 && !whole && at_end; }
 
 // The form for many rows (paged_tc.cu).
 int chunk_launch(const Params& p, int dtype, int dim, int ctas, cudaStream_t stream);

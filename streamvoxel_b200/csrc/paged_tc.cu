@@ -213,53 +213,6 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // Of every 8 pairs of exponentials, this many go to the FMA pipe.
 constexpr int kPolyPairs = 2;
 
-// A CTA's share, unit by unit: key tiles [t0, t1) of the unit at `at`; `part` counts the units of its run of the line (-1:
-// a unit dealt out whole).
-struct Walk {
-  Cursor at;
-  int t0, t1, waves, left, units, part;
-  __device__ __forceinline__ Walk(const Params& p, const Place& place) {
-    waves = place.waves;
-    left = place.count;
-    units = 0;
-    part = -1;
-    t0 = t1 = 0;
-    if (waves) {
-      at.first(p);
-      at.skip(p, blockIdx.x);
-      t1 = at.tiles;
-    } else {
-      start_run(p, place);
-    }
-  }
-  __device__ __forceinline__ void start_run(const Params& p, const Place& place) {
-    if (left <= 0) return;
-    part = 0;
-    at.set(p, place);
-    t0 = place.t;
-    t1 = min(at.tiles, t0 + left);
-  }
-  __device__ __forceinline__ bool more() const { return waves > 0 || left > 0; }
-  __device__ __forceinline__ void next(const Params& p, const Place& place) {
-    ++units;
-    if (waves) {
-      if (--waves) {
-        at.skip(p, gridDim.x);
-        t1 = at.tiles;
-      } else {
-        start_run(p, place);
-      }
-      return;
-    }
-    left -= t1 - t0;
-    if (left <= 0) return;
-    ++part;
-    at.next(p);
-    t0 = 0;
-    t1 = min(at.tiles, left);
-  }
-};
-
 // Live query tiles of a unit (tile_tokens tokens each).
 __device__ __forceinline__ int live_tiles(const Params& p, const Cursor& at, int tile_tokens) {
   return at.q.n - at.j * p.unit_tokens > tile_tokens ? 2 : 1;
@@ -339,7 +292,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     const uint64_t q = tc::sw128_desc(smem_addr(sq + i * C::q_bytes));
     int g = 0, n = 0;   // tiles of the ring and of this chain
     bool ok = true;
-    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
+    for (Walk w(p, place, cta); ok && w.more(); w.next(p, place, gridDim.x)) {
       const bool none = idle(w, i);
       if (!wait_w(q_full, w.units & 1, abort_flag)) break;
       for (int t = w.t0; t < w.t1; ++t, ++g) {
@@ -369,7 +322,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     const uint32_t d = tmem + C::o_col + 128 * i, a = tmem + C::s_col + 128 * i;
     int g = 0, n = 0;
     bool ok = true;
-    for (Walk w(p, place); ok && w.more(); w.next(p, place)) {
+    for (Walk w(p, place, cta); ok && w.more(); w.next(p, place, gridDim.x)) {
       const bool none = idle(w, i);
       for (int t = w.t0; t < w.t1; ++t, ++g) {
         const int s = g % C::stages;
@@ -397,7 +350,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
       uint64_t* empty = is_v ? v_empty : k_empty;
       uint8_t* ring = is_v ? sv : sk;
       const CUtensorMap* map = is_v ? &maps.v : &maps.k;
-      Walk w(p, place);
+      Walk w(p, place, cta);
       int g = 0, ends = 0;
       bool ok = true;
       // The page id of box `lane` of tile t, as the pool's coordinate.
@@ -425,7 +378,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
         }
         const Cursor at = w.at;
         const int t0 = w.t0, t1 = w.t1;
-        w.next(p, place);
+        w.next(p, place, gridDim.x);
         for (int t = t0; t < t1; ++t, ++g) {
           const int s = g % C::stages;
           if (g >= C::stages && !wait_w(empty + s, (g / C::stages - 1) & 1, abort_flag)) { ok = false; break; }
@@ -494,8 +447,8 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
   const bool in_tile = row < tile_tokens * p.group;
   int n0 = 0;
   bool ok = true;
-  Walk w(p, place);
-  for (; ok && w.more(); w.next(p, place)) {
+  Walk w(p, place, cta);
+  for (; ok && w.more(); w.next(p, place, gridDim.x)) {
     const Cursor& at = w.at;
     if (p.status && threadIdx.x == 128) {
       if (__ldg(p.lengths + at.s) != at.q.len) atomicOr(p.status + at.s, SVX_STATUS_BAD_PAGE);
@@ -591,7 +544,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     if (!ok) break;
     tc::fence_after();
     n0 += count;
-    const bool whole = w.t0 == 0 && w.t1 == at.tiles;
+    const bool whole = w.whole();
     // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
     // makes the row NaN, as inf - inf does.
     if (m_used == INFINITY) l_run = __int_as_float(0x7fffffff);
@@ -599,7 +552,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     const bool none = m_used == -INFINITY;
     const float factor = none ? 0.f : whole ? 1.f / l_run : 1.f;
     if (warp_live) {
-      const int64_t slot = 2 * cta + (w.part > 0 ? 1 : 0);
+      const int64_t slot = partial_slot(cta, w.part);
       const int part_row = i * TQ + row;
       float4* part = reinterpret_cast<float4*>(p.partial_o) + slot * p.rows * (D / 4) + part_row;
       const int64_t row0 = (int64_t)(at.q.row0 + at.j * p.unit_tokens) * p.q_heads + at.h * p.group;
@@ -653,7 +606,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
       if (live && whole && p.lse)
         p.lse[row0 + out_row] = none ? -INFINITY : (m_used - K::shift + log2f(l_run)) * 0.69314718056f;
     }
-    if (threadIdx.x == 128 && w.part == 0 && !whole && w.t1 == at.tiles)
+    if (threadIdx.x == 128 && ends_for_others(w.part, whole, w.t1 == at.tiles))
       p.join[cta] = Join{cta - place.first + 1, place.first, place.first_slot, at.q.row0 + at.j * p.unit_tokens,
                          min(p.unit_tokens, at.q.n - at.j * p.unit_tokens), at.h * p.group, p.group, 0};
     // O_i has been read; the next unit's first P V, which overwrites it, is issued only after this warpgroup's next
@@ -686,7 +639,6 @@ __device__ __forceinline__ void join_few_parts(const Params& p, const Join& join
   const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
   const bool live = r < p.rows && in_tile < p.tile_tokens * join.group && token < join.tokens;
   if (!__any_sync(0xffffffffu, live)) return;
-  auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)); };
   float top = -INFINITY, total = 0.f, f[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) f[j] = 0.f;
@@ -694,10 +646,10 @@ __device__ __forceinline__ void join_few_parts(const Params& p, const Join& join
     const float4* src = reinterpret_cast<const float4*>(p.partial_o) + c / 4 * p.rows + r;
 #pragma unroll 2
     for (int i = 0; i < join.parts; ++i) {   // the loads of two parts are on their way together
-      const float2 ml = p.partial_ml[slot(i) * p.rows + r];
+      const float2 ml = p.partial_ml[join.slot(i) * p.rows + r];
       float4 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = src[slot(i) * p.rows * (D / 4) + k * p.rows];
+      for (int k = 0; k < 8; ++k) v[k] = src[join.slot(i) * p.rows * (D / 4) + k * p.rows];
       const float now = fmaxf(top, ml.x);
       const float old = top == now ? 1.f : tc::ex2(top - now), x = ml.x == now ? 1.f : tc::ex2(ml.x - now);
       top = now;
@@ -738,7 +690,6 @@ __device__ __forceinline__ void join_many_parts(const Params& p, const Join& joi
   const int r = task / (D / 32) * 32 + lane, c = task % (D / 32) * 32, in_tile = r % p.tile_rows;
   const int token = r / p.tile_rows * p.tile_tokens + in_tile / join.group;
   const bool live = r < p.rows && in_tile < p.tile_tokens * join.group && token < join.tokens;
-  auto slot = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? join.first_slot : 0)); };
   float top = -INFINITY, total = 0.f;
   float4 f[8];
 #pragma unroll
@@ -747,10 +698,10 @@ __device__ __forceinline__ void join_many_parts(const Params& p, const Join& joi
     const float4* src = reinterpret_cast<const float4*>(p.partial_o) + c / 4 * p.rows + r;
 #pragma unroll 2
     for (int i = share; i < join.parts; i += 4) {   // the loads of two parts are on their way together
-      const float2 ml = p.partial_ml[slot(i) * p.rows + r];
+      const float2 ml = p.partial_ml[join.slot(i) * p.rows + r];
       float4 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = src[slot(i) * p.rows * (D / 4) + k * p.rows];
+      for (int k = 0; k < 8; ++k) v[k] = src[join.slot(i) * p.rows * (D / 4) + k * p.rows];
       const float now = fmaxf(top, ml.x);
       const float old = top == now ? 1.f : tc::ex2(top - now), x = ml.x == now ? 1.f : tc::ex2(ml.x - now);
       top = now;
