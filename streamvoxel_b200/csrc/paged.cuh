@@ -252,6 +252,11 @@ SVX_HOST_DEVICE int64_t dealt_whole(const Params& p, int c, int ctas, int waves)
   return tiles;
 }
 
+// Tiles of the run of a CTA that takes `dealt` tiles whole. full: the whole units of some CTA are an equal share already;
+// every share is then a tile longer, so that no run before the line's end is empty. A run in the middle of a unit counts as
+// one of its parts (Join), and an empty one would leave nothing where the joining kernel reads.
+SVX_HOST_DEVICE int64_t run_length(int64_t each, int64_t dealt, bool full) { return each + (full ? 1 : 0) - dealt; }
+
 // Where CTA c's run begins: tile `begin` of the line, which lies among the sequences [s0, s1); `before` tiles come before
 // them. line: the runs' begins where units are dealt out whole, null where every run is `each` tiles long.
 SVX_HOST_DEVICE void find_place(const Params& p, int s0, int s1, int64_t before, int64_t begin, int64_t each, int c,
@@ -326,7 +331,8 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
       if (!__syncthreads_or(dealt > each)) break;
       waves >>= 1;
     }
-    const int64_t need = tid < ctas ? each - dealt : 0;   // waves == 0: equal runs of the whole line
+    const bool full = __syncthreads_or(tid < ctas && dealt == each);
+    const int64_t need = tid < ctas ? run_length(each, dealt, full) : 0;   // waves == 0: equal runs of the whole line
     int64_t need_before, dealt_before, need_total, dealt_total;
     block_scan<kThreads, true>(need, dealt, sh, &need_before, &dealt_before, &need_total, &dealt_total);
     if (tid < ctas) scratch[tid] = min(total, dealt_total + need_before);
@@ -394,7 +400,7 @@ struct Walk {
 
 // Left by CTA c for the joining kernel, where its run ends a unit that an earlier CTA began: the unit's rows and heads,
 // the CTA that began it, and whether the unit was that CTA's first of the line (partial slot 2 first) or its last
-// (2 first + 1). The CTAs between hold their parts, like c, in their first slots.
+// (2 first + 1). The CTAs between hold their parts, like c, in their first slots: none of their runs is empty.
 struct Join {
   int parts;               // 0: nothing to join
   int first, first_slot;

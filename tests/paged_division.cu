@@ -43,7 +43,7 @@ extern "C" __attribute__((visibility("default"))) int paged_division(const int32
   int64_t at = dealt_total;
   for (int c = 0; c < ctas; ++c) {
     line[c] = at < total ? at : total;
-    at += each - dealt[c];
+    at += run_length(each, dealt[c], waves && most == each);
   }
   line[ctas] = total;
   counts[0] = 0;

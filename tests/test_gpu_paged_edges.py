@@ -1,0 +1,46 @@
+"""Edges of the rotary and paged-cache operators on the GPU: calls that their documentation allows and that once went wrong."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_reference as ref
+from test_gpu_paged import TYPES, _cache, _check, _fill, _offsets
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def ops():
+    from streamvoxel_b200 import _lib, ops
+    _lib.require_device()
+    return ops
+
+
+@pytest.fixture(autouse=True)
+def no_grad():
+    with torch.no_grad():
+        yield
+
+
+@pytest.mark.parametrize('news,lengths,heads,group,page,causal', [
+    ([512] * 16, [512] * 16, 8, 4, 64, True), ([753, 1163, 511], [820, 3847, 679], 4, 8, 64, True),
+    ([784, 768, 3184], [128, 320, 128], 1, 16, 16, False)])
+def test_whole_units_that_fill_a_share(ops, news, lengths, heads, group, page, causal):
+    """Batches in which the units that a CTA takes whole are its share exactly: nothing is joined that this call did not
+    write, whatever the workspace held before."""
+    rng, g = np.random.default_rng(23), torch.Generator().manual_seed(23)
+    k_pages, v_pages, table, lengths = _cache(rng, lengths, heads, page, 64, torch.bfloat16)
+    _fill((k_pages, v_pages), table, lengths, g)
+    offsets = _offsets(news)
+    q = torch.randn((sum(news), heads * group, 64), generator=g).bfloat16().cuda()
+    workspace = ops.paged_attention_workspace(sum(news), len(news), heads * group, heads, 64, 'cuda', max(news))
+    lse = torch.empty((sum(news), heads * group), device='cuda')
+    want, bound, want_lse, lse_bound, _ = ref.attention(q, k_pages, v_pages, table, lengths, offsets.cpu(), causal)
+    for fill in (255, 0, 0x7f):   # NaN, zeros, 3.4e38
+        workspace.fill_(fill)
+        got = ops.paged_attention(q, k_pages, v_pages, table, lengths, offsets, causal=causal, lse=lse,
+                                  max_query=max(news), workspace=workspace)
+        ref.close(got, want, bound)
+        ref.close(lse, want_lse, lse_bound)

@@ -122,3 +122,26 @@ def check_joins(segments, named):
         assert [left.get(slot) for slot in slots] == [unit] * len(slots), (unit, slots)
         assert slots == [slot for _, slot in sorted(parts[unit])]
     assert joined == set(parts)
+
+
+# An empty run between two CTAs that share a unit: the dealt units of a CTA in the middle fill its share exactly.
+FULL_SHARES = [dict(news=[512] * 16, lengths=[512] * 16, kv_heads=8, unit_tokens=64, causal=True),
+               dict(news=[753, 1163, 511], lengths=[820, 3847, 679], kv_heads=4, unit_tokens=32, causal=True),
+               dict(news=[784, 768, 3184], lengths=[128, 320, 128], kv_heads=1, unit_tokens=16, causal=False)]
+
+
+@pytest.mark.parametrize('batch', FULL_SHARES)
+def test_joins_of_full_shares(division, batch):
+    segments, named, waves = division(**batch)
+    assert waves > 0 and named
+    check_cover(segments, **batch)
+    check_joins(segments, named)
+
+
+def test_joins_read_what_their_units_left(division):
+    dealt = 0
+    for batch in batches(3000, 2):
+        segments, named, waves = division(**batch)
+        dealt += waves > 0
+        check_joins(segments, named)
+    assert dealt > 200
