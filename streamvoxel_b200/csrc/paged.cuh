@@ -215,12 +215,13 @@ struct Cursor {
   }
 };
 
-// Tiles and units of the sequences [s0, s1), all heads.
-SVX_HOST_DEVICE void add_sequences(const Params& p, int s0, int s1, int64_t* tiles, int64_t* units) {
+// Tiles and units of the sequences [s0, s1), all heads; *last: the last of them.
+SVX_HOST_DEVICE void add_sequences(const Params& p, int s0, int s1, int64_t* tiles, int64_t* units, Sequence* last) {
   const int heads = p.kv_heads * p.blocks;
   *tiles = *units = 0;
+  *last = Sequence{};
   for (int s = s0; s < s1; ++s) {
-    const Sequence q = load_sequence(p, s);
+    const Sequence q = *last = load_sequence(p, s);
     const int n = token_tiles(p, q);
     *tiles += tiles_before(p, q, n) * heads;
     *units += (int64_t)n * heads;
@@ -258,13 +259,14 @@ SVX_HOST_DEVICE int64_t dealt_whole(const Params& p, int c, int ctas, int waves)
 SVX_HOST_DEVICE int64_t run_length(int64_t each, int64_t dealt, bool full) { return each + (full ? 1 : 0) - dealt; }
 
 // Where CTA c's run begins: tile `begin` of the line, which lies among the sequences [s0, s1); `before` tiles come before
-// them. line: the runs' begins where units are dealt out whole, null where every run is `each` tiles long.
-SVX_HOST_DEVICE void find_place(const Params& p, int s0, int s1, int64_t before, int64_t begin, int64_t each, int c,
-                                const int64_t* line, Place* place) {
+// them and `last` is the last of them. line: the runs' begins where units are dealt out whole, null where every run is
+// `each` tiles long.
+SVX_HOST_DEVICE void find_place(const Params& p, int s0, int s1, const Sequence& last, int64_t before, int64_t begin,
+                                int64_t each, int c, const int64_t* line, Place* place) {
   const int heads = p.kv_heads * p.blocks;
   int64_t at = before;
   for (int s = s0; s < s1; ++s) {
-    const Sequence q = load_sequence(p, s);
+    const Sequence q = s + 1 < s1 ? load_sequence(p, s) : last;
     const int n = token_tiles(p, q);
     const int64_t head = tiles_before(p, q, n);
     if (begin < at + head * heads) {
@@ -309,7 +311,8 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
   const int id = few ? lane_id() : tid, per = few ? 1 : (p.sequences + kThreads - 1) / kThreads;
   const int s0 = min(p.sequences, id * per), s1 = min(p.sequences, s0 + per);
   int64_t tiles, units, before, units_before, total, units_total;
-  add_sequences(p, s0, s1, &tiles, &units);
+  Sequence last;
+  add_sequences(p, s0, s1, &tiles, &units, &last);
   if (few) {
     before = warp_scan(tiles);
     units_before = kWaves ? warp_scan(units) : 0;
@@ -346,7 +349,7 @@ __device__ __forceinline__ void plan(const Params& p, int c, int ctas, PlanShare
     sh.place.count = (int)(end - begin);
   }
   if (begin < end && begin >= before && begin < before + tiles && (!few || tid < 32))
-    find_place(p, s0, s1, before, begin, each, c, kWaves && waves ? scratch : nullptr, &sh.place);
+    find_place(p, s0, s1, last, before, begin, each, c, kWaves && waves ? scratch : nullptr, &sh.place);
   __syncthreads();
 }
 

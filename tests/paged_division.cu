@@ -23,7 +23,8 @@ extern "C" __attribute__((visibility("default"))) int paged_division(const int32
   int64_t units_total = 0;
   for (int s = 0; s < p.sequences; ++s) {
     int64_t tiles, units;
-    add_sequences(p, s, s + 1, &tiles, &units);
+    Sequence last;
+    add_sequences(p, s, s + 1, &tiles, &units, &last);
     before[s + 1] = before[s] + tiles;
     units_total += units;
   }
@@ -56,7 +57,7 @@ extern "C" __attribute__((visibility("default"))) int paged_division(const int32
     if (place.count > 0) {
       int s = 0;
       while (before[s + 1] <= line[c]) ++s;
-      find_place(p, s, s + 1, before[s], line[c], each, c, waves ? line.data() : nullptr, &place);
+      find_place(p, s, s + 1, load_sequence(p, s), before[s], line[c], each, c, waves ? line.data() : nullptr, &place);
     }
     for (Walk w(p, place, c); w.more(); w.next(p, place, ctas)) {
       if (rows == segment_rows) return -1;
