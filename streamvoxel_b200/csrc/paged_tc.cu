@@ -90,6 +90,8 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile ui
     }
   }
 }
+// Warp-collective: the lanes agree on the outcome, so that none leaves a loop of warp-wide instructions alone where `abort`
+// is raised while the phase completes. Every wait of the kernel's loops goes through it.
 __device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
   return __all_sync(0xffffffffu, wait(bar, parity, abort));
 }
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
   // Tile n of a chain (counted over the CTA's whole run) uses buffer n % 2, whose barriers are in phase n / 2. With one
   // barrier for both buffers a wait could find the phase two tiles back and take it for its own.
   auto buffer_wait = [&](uint64_t* bars, int i, int n) {
-    return wait(bars + 2 * i + (n & 1), (n >> 1) & 1, abort_flag);
+    return wait_w(bars + 2 * i + (n & 1), (n >> 1) & 1, abort_flag);
   };
   const int warp = warp_id(), lane = lane_id(), cta = blockIdx.x;
   const int tile_tokens = p.tile_tokens;
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
           continue;
         }
         // S(n) goes where P(n - 2) was
-        ok = n < 2 || __all_sync(0xffffffffu, buffer_wait(pv_done, i, n - 2));
+        ok = n < 2 || buffer_wait(pv_done, i, n - 2);
         if (!ok) break;
         tc::fence_after();
         issue_scores<D>(d + 64 * (n & 1), q, tc::sw128_desc(smem_addr(sk + s * C::k_bytes)), idesc,
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
           if (lane == 0) tc::mbar_arrive(v_empty + s);
           continue;
         }
-        ok = __all_sync(0xffffffffu, buffer_wait(p_full, i, n));
+        ok = buffer_wait(p_full, i, n);
         if (!ok) break;
         tc::fence_after();
         issue_values(d, a + 64 * (n & 1), tc::sw128_desc(smem_addr(sv + s * C::k_bytes), C::k_atom, 1024), idesc, t != w.t0,
@@ -426,6 +428,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     asm volatile("barrier.sync 1, %0;" ::"n"(kThreads) : "memory");
     if (warp == 1) {
       mbar_wait(drained, 0);
+      __syncwarp();
       tc::fence_after();
       tc::tmem_dealloc(*tmem_slot, C::tmem_cols);
     }
@@ -540,7 +543,6 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
       if (lane == 0) tc::mbar_arrive(p_full + 2 * i + buffer);
     }
     if (ok) ok = buffer_wait(pv_done, i, n0 + count - 1);
-    ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     tc::fence_after();
     n0 += count;
