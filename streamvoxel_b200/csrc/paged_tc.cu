@@ -196,10 +196,15 @@ __device__ __forceinline__ float max2_nan(float a, float b) {
 }
 
 // 2^x on the FMA pipe for a pair: x = j + f with j = rint(x) from the 1.5 * 2^23 magic sum, a degree-4 polynomial fitted
-// to 2^f on [-0.5, 0.5] (relative error 2.7e-6), j added to the exponent field; x is clamped at -125.5.
+// to 2^f on [-0.5, 0.5] (relative error 2.7e-6), times 2^j. x is clamped at -127, which gives exactly 0, so that hidden keys
+// (-inf) and weights under 2^-127 add nothing, however large the value behind them. kProduct: a product with 2^j, made in
+// the exponent field and 0 there; else j added to the exponent field, the sums that fall below it cut to 0 (between 2^-127
+// and 2^-126 the fraction is lost). The first is faster with two query tiles a unit (attn-chunk 1,210 us against 1,248,
+// attn-windows 184 against 186), the second with one, where registers are short (attn-verify 60.5 against 62.3).
+template <bool kProduct>
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -125.5f);
-  x.y = fmaxf(x.y, -125.5f);
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
   const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
   const float2 j = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
   const float2 f = __ffma2_rn(j, make_float2(-1.f, -1.f), x);
@@ -208,8 +213,11 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   q = __ffma2_rn(q, f, make_float2(0.240247443318367f, 0.240247443318367f));
   q = __ffma2_rn(q, f, make_float2(0.6931218504905701f, 0.6931218504905701f));
   q = __ffma2_rn(q, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+  if (kProduct)
+    return __fmul2_rn(q, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                     __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+  return make_float2(__int_as_float(max(0, __float_as_int(q.x) + (__float_as_int(t.x) << 23))),
+                     __int_as_float(max(0, __float_as_int(q.y) + (__float_as_int(t.y) << 23))));
 }
 
 // Of every 8 pairs of exponentials, this many go to the FMA pipe.
@@ -517,7 +525,7 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
       for (int j = 0; j < TK; j += 2) {
         const int c = j >> 5, jj = j & 31;
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[c][jj]), __uint_as_float(r[c][jj + 1])), scale2, nbase2);
-        const float2 e = ((j >> 1) & 7) < kPolyPairs ? exp2_poly(x) : make_float2(tc::ex2(x.x), tc::ex2(x.y));
+        const float2 e = ((j >> 1) & 7) < kPolyPairs ? exp2_poly<kChains == 2>(x) : make_float2(tc::ex2(x.x), tc::ex2(x.y));
         acc[(j >> 1) & 3] = __fadd2_rn(acc[(j >> 1) & 3], e);
         packed[j >> 1] = K::pack(e.x, e.y);
       }
@@ -547,10 +555,8 @@ __global__ void __launch_bounds__(Tiles<D, kChains>::threads, 3 - kChains)
     tc::fence_after();
     n0 += count;
     const bool whole = w.whole();
-    // A row without keys in these tiles has sums of 2^-125 from the clamped exponentials: nothing. An infinite score
-    // makes the row NaN, as inf - inf does.
+    // An infinite score makes the row NaN, as inf - inf does.
     if (m_used == INFINITY) l_run = __int_as_float(0x7fffffff);
-    if (m_used == -INFINITY) l_run = 0.f;
     const bool none = m_used == -INFINITY;
     const float factor = none ? 0.f : whole ? 1.f / l_run : 1.f;
     if (warp_live) {

@@ -44,3 +44,26 @@ def test_whole_units_that_fill_a_share(ops, news, lengths, heads, group, page, c
                                   max_query=max(news), workspace=workspace)
         ref.close(got, want, bound)
         ref.close(lse, want_lse, lse_bound)
+
+
+@pytest.mark.parametrize('news', [5, 60, 200])   # one form of the kernel each
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('kind', ['hidden', 'far below'])
+def test_values_without_weight_count_nothing(ops, dtype, news, kind):
+    """Values near the type's largest behind keys that the mask hides, or whose weight is under 2^-200, add nothing."""
+    rng, g, dtype = np.random.default_rng(20), torch.Generator().manual_seed(20), TYPES[dtype]
+    keys, dim, last = 300, 64, 20 if news > 20 else 2
+    k_pages, v_pages, table, lengths = _cache(rng, [keys], 2, 16, dim, dtype)
+    _fill((k_pages, v_pages), table, lengths, g)
+    largest = 2.0 ** 127 if dtype == torch.bfloat16 else 2.0 ** 15
+    q = torch.randn((news, 2, dim), generator=g).to(dtype).cuda()
+    q[..., 0] = 1
+    for place in range(keys - last, keys):
+        v_pages[int(table[0, place // 16]), :, place % 16] = largest
+        if kind != 'hidden':
+            k_pages[int(table[0, place // 16]), :, place % 16, 0] = -1200   # scores of -150
+    args = q, k_pages, v_pages, table, lengths, _offsets([news])
+    got = ops.paged_attention(*args, causal=kind == 'hidden', max_query=news)
+    want, bound = ref.attention(*args[:5], args[5].cpu(), kind == 'hidden')[:2]
+    rows = news - last if kind == 'hidden' else news   # the last rows see those values
+    ref.close(got[:rows], want[:rows], bound[:rows])
