@@ -343,6 +343,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::ctas_per_sm) few_rows_kern
         sum.x = fmaf(v.x, f[x], sum.x); sum.y = fmaf(v.y, f[x], sum.y);
         sum.z = fmaf(v.z, f[x], sum.z); sum.w = fmaf(v.w, f[x], sum.w);
       }
+      // A row without keys: its weights of 0 have made NaN of infinite values that other rows of the unit see.
+      if (sum_r == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (!whole) {
         *reinterpret_cast<float4*>(p.partial_o + (slot * p.rows + r) * D + k * 32 + c) = sum;
       } else if (live) {

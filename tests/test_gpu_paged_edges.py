@@ -67,3 +67,19 @@ def test_values_without_weight_count_nothing(ops, dtype, news, kind):
     want, bound = ref.attention(*args[:5], args[5].cpu(), kind == 'hidden')[:2]
     rows = news - last if kind == 'hidden' else news   # the last rows see those values
     ref.close(got[:rows], want[:rows], bound[:rows])
+
+
+@pytest.mark.parametrize('news,length,hint', [(5, 2, 5), (16, 3, 16), (40, 7, 40), (40, 7, 1), (300, 30, 300)])
+def test_rows_without_keys_take_nothing_from_their_neighbours(ops, news, length, hint):
+    """Fewer keys than new tokens: the first rows see none and give 0, whatever the values of the others' keys are."""
+    rng, g = np.random.default_rng(21), torch.Generator().manual_seed(21)
+    k_pages, v_pages, table, lengths = _cache(rng, [length], 1, 16, 64, torch.bfloat16)
+    _fill((k_pages, v_pages), table, lengths, g)
+    v_pages[int(table[0, 0]), :, :length] = math.nan
+    v_pages[int(table[0, 0]), :, 0] = math.inf
+    q = torch.randn((news, 1, 64), generator=g).bfloat16().cuda()
+    lse = torch.zeros((news, 1), device='cuda')
+    out = ops.paged_attention(q, k_pages, v_pages, table, lengths, _offsets([news]), lse=lse, max_query=hint)
+    none = news - length
+    assert bool((out[:none] == 0).all()) and bool((lse[:none] == -math.inf).all())
+    assert not bool(out[none:].isfinite().any()) and bool(lse[none:].isfinite().all())
