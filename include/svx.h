@@ -290,7 +290,8 @@ typedef struct {
 
 /* out = rotation of x, both [tokens][heads][dim] of fp32, bf16 or fp16 with strides in elements (values of a head are
  * contiguous); values past rot are copied. inverse != 0: the transposed rotation, which takes a gradient of out to the
- * gradient of x. Angles are formed in float64, values computed in fp32 and rounded once. out may be x. */
+ * gradient of x. Angles are formed in float64 (an angle a is off by up to 2^-51 |a|: to 32 bits up to 2^27 radians; any
+ * finite position gives a rotation), values computed in fp32 and rounded once. out may be x. */
 SVX_API int svx_rope(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, void* out,
                      int64_t out_token_stride, int64_t out_head_stride, int tokens, int heads, int dim,
                      const svx_rotary* rotary, int inverse, void* stream);

@@ -128,8 +128,11 @@ __device__ __forceinline__ void turn_across(uint4& a, uint4& b, const float2* cs
 }
 
 // (cos, sin) of 2 pi turns. The turns are reduced to [-1/8, 1/8] in float64, then sine and cosine are their Taylor series up
-// to x^9 and x^10 (|x| <= pi / 4: the next terms are under 2e-9), and the quarter turns swap and negate them.
+// to x^9 and x^10 (|x| <= pi / 4: the next terms are under 2e-9), and the quarter turns swap and negate them. Turns from
+// 2^49 on, whose eighths float64 does not hold, are reduced to a turn first: the angle means nothing there, but the pair
+// still turns (beyond |x| = pi / 4 the series grow without limit).
 __device__ __forceinline__ float2 cos_sin_turns(double turns) {
+  if ((__double2hiint(turns) & 0x7fffffff) >= (1023 + 49) << 20) turns -= rint(turns);
   // Adding 1.5 * 2^52 rounds to a whole number, which then stands in the low bits (|turns| < 2^49); a rounding and a
   // conversion to integers would take the slow conversion pipe.
   const double sum = fma(4.0, turns, 6755399441055744.0), quarters = sum - 6755399441055744.0;

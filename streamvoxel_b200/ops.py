@@ -437,7 +437,7 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
     token and head strides free) turned by positions * inv_freq and multiplied by scale, the others copied.
 
     positions: [tokens], or [tokens, axes] with the pairs split evenly among the axes (int32, int64 or float32). inv_freq:
-    float64, from `rope_frequencies`. Pairs are (2j, 2j + 1) ('interleaved') or (j, j + rot / 2) ('half'). inverse: the
+    float64, from `rope_frequencies`. Angles are formed in float64: an angle a is off by up to 2^-51 |a|. Pairs are (2j, 2j + 1) ('interleaved') or (j, j + rot / 2) ('half'). inverse: the
     transposed rotation, the gradient's way back; x that requires grad takes it by itself. out: a [tokens, heads, dim]
     tensor of x's type, x itself or one that does not overlap it."""
     if x.ndim != 3:

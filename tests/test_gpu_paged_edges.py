@@ -83,3 +83,18 @@ def test_rows_without_keys_take_nothing_from_their_neighbours(ops, news, length,
     none = news - length
     assert bool((out[:none] == 0).all()) and bool((lse[:none] == -math.inf).all())
     assert not bool(out[none:].isfinite().any()) and bool(lse[none:].isfinite().all())
+
+
+@pytest.mark.parametrize('layout', ['interleaved', 'half'])
+@pytest.mark.parametrize('positions', [torch.tensor([2 ** 50, 2 ** 54 + 4, -2 ** 62 + 512, 2 ** 63 - 1]),
+                                       torch.tensor([1e17, -3e20, 1e30, 3e38])])
+def test_rope_of_any_position_is_a_rotation(ops, positions, layout):
+    """Positions past what float64 angles resolve still turn every pair without changing its length."""
+    freq, _ = ops.rope_frequencies(64)
+    x = torch.randn((4, 3, 64), generator=torch.Generator().manual_seed(22)).cuda()
+    y = ops.rope(x, positions.cuda(), freq, layout=layout).double()
+    pair = (lambda t: t.unflatten(-1, (2, 32)).movedim(-2, -1)) if layout == 'half' else \
+        (lambda t: t.unflatten(-1, (32, 2)))
+    before, after = pair(x.double()).norm(dim=-1), pair(y).norm(dim=-1)
+    # cosine and sine within 2^-22 each, two products and a sum: 2^-21 of |a| + |b| a value, two values, |a| + |b| <= 1.5 r
+    assert bool(((after - before).abs() <= 2.0 ** -19 * before).all())
