@@ -9,6 +9,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from streamvoxel_b200 import _lib
 from streamvoxel_b200._lib import check, ptr, stream_ptr
@@ -438,7 +439,8 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
 
     positions: [tokens], or [tokens, axes] with the pairs split evenly among the axes (int32, int64 or float32). inv_freq:
     float64, from `rope_frequencies`. Angles are formed in float64: an angle a is off by up to 2^-51 |a|. Pairs are (2j, 2j + 1) ('interleaved') or (j, j + rot / 2) ('half'). inverse: the
-    transposed rotation, the gradient's way back; x that requires grad takes it by itself. out: a [tokens, heads, dim]
+    transposed rotation, the gradient's way back; x that requires grad takes it by itself (positions and inv_freq have no
+    gradient, x no forward-mode derivative: refused). out: a [tokens, heads, dim]
     tensor of x's type, x itself or one that does not overlap it."""
     if x.ndim != 3:
         raise ValueError('x must be [tokens, heads, dim]')
@@ -452,6 +454,9 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
         raise ValueError('rope needs positions')
     strides = _rows('x', x, tokens, heads, dim, dtype)
     rotary = _rotary(inv_freq, positions, tokens, dim, layout, scale)
+    _constant('rope has no gradient for positions, inv_freq or out', positions, inv_freq, out)
+    if _forward_mode() and _has_tangent(x):
+        raise ValueError('rope has no forward-mode derivative; rotate the tangent by a call of its own')
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError('out is not available for x that requires grad')
@@ -470,6 +475,27 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
     if status:
         check(status, 'svx_rope')
     return out
+
+
+def _forward_mode():
+    """Whether tensors may carry forward-mode tangents at present."""
+    return getattr(forward_ad, '_current_level', 0) >= 0
+
+
+def _has_tangent(t):
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
+def _constant(what, *tensors):
+    """Refuse tensors whose derivative would be lost: those that require grad, or carry a forward-mode tangent."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(what)
+    if _forward_mode():
+        for t in tensors:
+            if t is not None and _has_tangent(t):
+                raise ValueError(what)
 
 
 def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
@@ -500,10 +526,7 @@ def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
                            sequences, width, table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(), status)
 
 
-def _no_grad(*tensors):
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError('the paged cache takes no part in autograd: call under torch.no_grad()')
+_CACHE_GRAD = 'the paged cache takes no part in autograd: detach its operands or call under torch.no_grad()'
 
 
 def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=None, positions=None,
@@ -521,7 +544,7 @@ def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=No
     dtype, heads, dim, tokens = k_pages.dtype, cache.kv_heads, cache.dim, len(k)
     k_strides = _rows('k', k, tokens, heads, dim, dtype)
     v_strides = _rows('v', v, tokens, heads, dim, dtype)
-    _no_grad(k, v, k_pages, v_pages, q)
+    _constant(_CACHE_GRAD, k, v, k_pages, v_pages, inv_freq, positions, q, q_out)
     index = _index_of(k_pages, v_pages, table, lengths, offsets, k, v, inv_freq, positions, q, q_out, status)
     rotary = None
     if inv_freq is not None:
@@ -588,7 +611,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
         max_query = 0
     elif max_query < 0:
         raise ValueError('max_query must not be negative')
-    _no_grad(q, k_pages, v_pages)
+    _constant(_CACHE_GRAD, q, k_pages, v_pages, out, lse)
     index = _index_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
