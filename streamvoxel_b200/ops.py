@@ -10,6 +10,7 @@ import math
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from streamvoxel_b200 import _lib
 from streamvoxel_b200._lib import check, ptr, stream_ptr
@@ -461,6 +462,7 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
         if out is not None:
             raise ValueError('out is not available for x that requires grad')
         return _Rope.apply(x, positions, inv_freq, layout, scale, inverse)
+    given = out
     if out is None:
         index = _index_of(x, positions, inv_freq)
         out = x.new_empty((tokens, heads, dim))
@@ -474,6 +476,8 @@ def rope(x, positions, inv_freq, *, layout='interleaved', scale=1.0, inverse=Fal
                         *out_strides, tokens, heads, dim, ctypes.byref(rotary), bool(inverse))
     if status:
         check(status, 'svx_rope')
+    if given is not None:
+        increment_version(given)
     return out
 
 
@@ -496,6 +500,11 @@ def _constant(what, *tensors):
         for t in tensors:
             if t is not None and _has_tangent(t):
                 raise ValueError(what)
+
+
+def _written(*tensors):
+    """Tell autograd that these were written, so that a backward pass that saved one of them says so."""
+    increment_version([t for t in tensors if t is not None])
 
 
 def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
@@ -567,10 +576,11 @@ def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=No
             if not q_out.is_contiguous():
                 raise ValueError('q_out must be contiguous')
         queries = q.data_ptr(), *q_strides, q_heads, q_out.data_ptr()
-    status = _launch_on(index, _lib.load().svx_paged_append, ctypes.byref(cache), k.data_ptr(), *k_strides, v.data_ptr(),
-                        *v_strides, tokens, rotary, *queries)
-    if status:
-        check(status, 'svx_paged_append')
+    code = _launch_on(index, _lib.load().svx_paged_append, ctypes.byref(cache), k.data_ptr(), *k_strides, v.data_ptr(),
+                      *v_strides, tokens, rotary, *queries)
+    if code:
+        check(code, 'svx_paged_append')
+    _written(k_pages, v_pages, q_out, status)
     return q_out
 
 
@@ -613,6 +623,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
         raise ValueError('max_query must not be negative')
     _constant(_CACHE_GRAD, q, k_pages, v_pages, out, lse)
     index = _index_of(q, k_pages, v_pages, table, lengths, offsets, out, lse, workspace, status)
+    given = out
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -632,8 +643,10 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
         workspace = q.new_empty((size,), dtype=torch.uint8)
     elif workspace.dtype != torch.uint8 or workspace.numel() < size or not workspace.is_contiguous():
         raise ValueError(f'workspace must be a contiguous uint8 tensor of at least {size} bytes')
-    status = _launch_on(index, lib.svx_paged_attention, ctypes.byref(cache), q.data_ptr(), *strides, tokens, heads, bool(causal),
-                        scale, out.data_ptr(), None if lse is None else lse.data_ptr(), max_query, workspace.data_ptr())
-    if status:
-        check(status, 'svx_paged_attention')
+    code = _launch_on(index, lib.svx_paged_attention, ctypes.byref(cache), q.data_ptr(), *strides, tokens, heads, bool(causal),
+                      scale, out.data_ptr(), None if lse is None else lse.data_ptr(), max_query, workspace.data_ptr())
+    if code:
+        check(code, 'svx_paged_attention')
+    if given is not None or lse is not None or status is not None:
+        _written(given, lse, status)
     return out

@@ -98,3 +98,60 @@ def test_rope_of_any_position_is_a_rotation(ops, positions, layout):
     before, after = pair(x.double()).norm(dim=-1), pair(y).norm(dim=-1)
     # cosine and sine within 2^-22 each, two products and a sum: 2^-21 of |a| + |b| a value, two values, |a| + |b| <= 1.5 r
     assert bool(((after - before).abs() <= 2.0 ** -19 * before).all())
+
+
+def _saved(tensor):
+    """A product whose backward pass needs `tensor` as it is now."""
+    with torch.enable_grad():
+        leaf = torch.ones_like(tensor, requires_grad=True)
+        return (leaf * tensor).sum()
+
+
+def _spoilt(product):
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        product.backward()
+
+
+def test_written_tensors_spoil_backward_passes_that_saved_them(ops):
+    """Outputs that the caller hands in, and the pools, are in-place writes for autograd."""
+    rng, g = np.random.default_rng(24), torch.Generator().manual_seed(24)
+    freq, _ = ops.rope_frequencies(64)
+    x, positions = torch.randn((4, 2, 64), generator=g).cuda(), torch.arange(4, device='cuda')
+    untouched, packed = _saved(x), torch.randn((4, 6, 64), generator=g).cuda()
+    product = _saved(packed)
+    ops.rope(x, positions, freq, out=packed[:, 2:4])   # a view of the saved tensor
+    _spoilt(product)
+    product = _saved(x)
+    ops.rope(x, positions, freq)
+    untouched.backward()
+    product.backward()
+    k_pages, v_pages, table, lengths = _cache(rng, [4], 2, 16, 64, torch.bfloat16, fill=0.0)
+    k, v = (torch.randn((4, 2, 64), generator=g).bfloat16().cuda() for _ in range(2))
+    q_out, args = torch.zeros_like(k), (k_pages, v_pages, table, lengths, _offsets([4]))
+    products = [_saved(t) for t in (k_pages, v_pages, q_out)]
+    ops.paged_append(k, v, *args, inv_freq=freq, q=k, q_out=q_out)
+    for product in products:
+        _spoilt(product)
+    out, lse = torch.zeros_like(k), torch.zeros((4, 2), device='cuda')
+    products = [_saved(t) for t in (out, lse)]
+    kept = _saved(k_pages)
+    ops.paged_attention(k, *args, out=out, lse=lse)
+    for product in products:
+        _spoilt(product)
+    kept.backward()   # the pools were only read
+
+
+def test_tensors_of_inference_mode(ops):
+    """Pools and outputs made under inference mode, which have no version, are written in and outside of it."""
+    rng, g = np.random.default_rng(25), torch.Generator().manual_seed(25)
+    freq, _ = ops.rope_frequencies(64)
+    with torch.inference_mode():
+        k_pages, v_pages, table, lengths = _cache(rng, [4], 2, 16, 64, torch.bfloat16, fill=0.0)
+        k = torch.randn((4, 2, 64), generator=g).bfloat16().cuda()
+        args = (k_pages, v_pages, table, lengths, _offsets([4]))
+        out = torch.zeros_like(k)
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            q = ops.paged_append(k, k, *args, inv_freq=freq, q=k)
+            assert ops.paged_attention(q, *args, out=out) is out
+            assert ops.rope(out, torch.arange(4, device='cuda'), freq, out=out) is out
