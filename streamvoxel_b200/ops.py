@@ -320,7 +320,11 @@ def attention(q, k, v, slots, heads, queries, keys, *, q_row_stride, kv_slot_str
 # ------------------------------------------------------------------------- rotary positions and the paged cache
 
 _ROW_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_F32_MAX = torch.finfo(torch.float32).max
 _POSITION_DTYPES = {torch.int32: _lib.I32, torch.int64: _lib.I64, torch.float32: _lib.F32}
+
+
+_INT_MAX = 2 ** 31 - 1   # the library's sizes; ctypes cuts larger ones without a word
 
 
 def _need(ok, text):
@@ -362,6 +366,8 @@ def _rows(name, t, tokens, heads, dim, dtype):
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f'{name} must be [tokens, heads, dim]')
+    if tokens > _INT_MAX or heads > _INT_MAX:
+        raise ValueError(f'{name} has sizes past 32 bits: {tuple(shape)}')
     if shape[0] != tokens or shape[1] != heads or shape[2] != dim:
         raise ValueError(f'{name} is {tuple(shape)}, expected {(tokens, heads, dim)}')
     if t.dtype != dtype:
@@ -381,8 +387,8 @@ def _rotary(inv_freq, positions, tokens, dim, layout, scale):
     if layout not in _lib.ROPE_LAYOUTS:
         raise ValueError(f'layout must be one of {sorted(_lib.ROPE_LAYOUTS)}')
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError('the rotary scale must be finite')
+    if not abs(scale) <= _F32_MAX:
+        raise ValueError('the rotary scale must be finite in 32 bits')
     if positions is None:
         return _lib.Rotary(inv_freq.data_ptr(), 2 * pairs, _lib.ROPE_LAYOUTS[layout], 1, scale, None, _lib.I64)
     shape = positions.shape
@@ -514,12 +520,16 @@ def _paged_cache(k_pages, v_pages, table, lengths, offsets, status):
     if dtype != torch.bfloat16 and dtype != torch.float16:
         raise ValueError(f'the cache must be bf16 or fp16, got {dtype}')
     pages, heads, page, dim = shape
+    if not (0 < pages <= _INT_MAX and 0 < heads <= 1024):
+        raise ValueError(f'the pools need pages and 1 to 1024 heads, got {tuple(shape)}')
     if page not in (16, 32, 64, 128, 256, 512, 1024):
         raise ValueError(f'a page must hold 16, 32, .. 1024 keys, got {page}')
     shape = table.shape
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError('table must be [sequences, pages of a sequence]')
     sequences, width = shape
+    if sequences > 1 << 20 or width * page > 1 << 30:
+        raise ValueError(f'table {tuple(shape)} is past 2^20 sequences or 2^30 keys a sequence')
     if lengths.ndim != 1 or len(lengths) != sequences or offsets.ndim != 1 or len(offsets) != sequences + 1:
         raise ValueError(f'lengths must be [{sequences}] and offsets [{sequences + 1}]')
     if not table.dtype == lengths.dtype == offsets.dtype == torch.int32:
@@ -554,12 +564,12 @@ def paged_append(k, v, k_pages, v_pages, table, lengths, offsets, *, inv_freq=No
     k_strides = _rows('k', k, tokens, heads, dim, dtype)
     v_strides = _rows('v', v, tokens, heads, dim, dtype)
     _constant(_CACHE_GRAD, k, v, k_pages, v_pages, inv_freq, positions, q, q_out)
-    index = _index_of(k_pages, v_pages, table, lengths, offsets, k, v, inv_freq, positions, q, q_out, status)
     rotary = None
     if inv_freq is not None:
         rotary = ctypes.byref(_rotary(inv_freq, positions, tokens, dim, layout, rope_scale))
     elif q is not None or positions is not None:
         raise ValueError('q and positions need inv_freq')
+    index = _index_of(k_pages, v_pages, table, lengths, offsets, k, v, inv_freq, positions, q, q_out, status)
     if q is None:
         if q_out is not None:
             raise ValueError('q_out needs q')

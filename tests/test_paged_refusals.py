@@ -58,3 +58,53 @@ def test_rope_refuses_forward_mode():
         args['x'] = forward_ad.make_dual(args['x'], torch.ones_like(args['x']))
         with pytest.raises(ValueError, match='forward-mode'):
             ops.rope(**args)
+
+
+def _far(shape, like):
+    """A tensor of that shape without memory behind it (strides 0)."""
+    return torch.zeros([1] * len(shape), dtype=like.dtype).expand(shape)
+
+
+@pytest.mark.parametrize('shape', [(2 ** 31, 2, 64), (2 ** 32 + 4, 2, 64), (4, 2 ** 32 + 2, 64)])
+def test_rope_refuses_sizes_past_32_bits(shape):
+    args = _rope_args()
+    args['x'] = _far(shape, args['x'])
+    with pytest.raises(ValueError, match='past 32 bits'):
+        ops.rope(**args)
+
+
+def test_append_refuses_sizes_past_32_bits():
+    args = _append_args()
+    args['k'] = args['v'] = _far((2 ** 32 + 2, 2, 64), args['k'])
+    with pytest.raises(ValueError, match='past 32 bits'):
+        ops.paged_append(**args)
+
+
+def test_attention_refuses_sizes_past_32_bits():
+    args = _attention_args()
+    args['q'] = _far((2 ** 32 + 2, 4, 64), args['q'])
+    with pytest.raises(ValueError, match='past 32 bits'):
+        ops.paged_attention(**args)
+
+
+@pytest.mark.parametrize('call,make', [(ops.paged_append, _append_args), (ops.paged_attention, _attention_args)])
+@pytest.mark.parametrize('change,reason', [
+    (dict(table=(2 ** 20 + 1, 3), lengths=(2 ** 20 + 1,), offsets=(2 ** 20 + 2,)), 'sequences'),
+    (dict(table=(2, 2 ** 32 + 3)), 'keys a sequence'), (dict(table=(2, 2 ** 26 + 1)), 'keys a sequence'),
+    (dict(k_pages=(6, 0, 16, 64), v_pages=(6, 0, 16, 64)), 'heads'),
+    (dict(k_pages=(6, 1025, 16, 64), v_pages=(6, 1025, 16, 64)), 'heads'),
+    (dict(k_pages=(0, 2, 16, 64), v_pages=(0, 2, 16, 64)), 'pages')])
+def test_caches_refuse_sizes(call, make, change, reason):
+    args = make()
+    for name, shape in change.items():
+        args[name] = _far(shape, args[name])
+    with pytest.raises(ValueError, match=reason):
+        call(**args)
+
+
+@pytest.mark.parametrize('scale', [1e39, -1e39, float('inf'), float('nan')])
+def test_rotary_scales_are_finite_in_32_bits(scale):
+    with pytest.raises(ValueError, match='finite'):
+        ops.rope(**_rope_args(), scale=scale)
+    with pytest.raises(ValueError, match='finite'):
+        ops.paged_append(**_append_args(), rope_scale=scale)
