@@ -490,10 +490,16 @@ int divide(int tokens, int sequences, int group, int dim, int max_query, bool ch
     d->tile_tokens = 128 / group;
     // Query tiles of a unit, and then one or two CTAs a SM. Two share the keys' way to the SM (16 chunks of 512 tokens x 4
     // heads of 128 over 4000 keys: 530 us against 673); one wastes less on chunks that fit a tile (32 of 5
-    // tokens x 8 heads of 128: 62 us against 83), and where the longest chunk is far above the mean, most do (1 to 700
-    // tokens x 6 heads of 64: 90 us against 99).
+    // tokens x 8 heads of 128: 62 us against 83). Where the longest chunk is far above the mean, most sequences are short
+    // and leave half of a two-tile CTA idle, even beside one long chunk. One tile against two, group 4 of 128 unless said:
+    //   mean of at most 3 tiles: 8192 tokens and 255 single ones 965 us against 1107, 4 x 2000 and 200 single 639 against
+    //   706, 64 sequences of one or 300 204 against 241, 16 of 1 to 2000 64 against 76; but 2000 and 31 single 184 against 150;
+    //   3 to 8 tiles: 100 of 1 to 700 tokens 648 against 598, 100 of 1 to 2048 1550 against 1389, 2 x 2000 and 30 single
+    //   (group 8) 218 against 189, 24 of 1 to 700 159 against 171; with 64-wide heads, which load half as much for each
+    //   product, 64 of 1 to 300 (group 6) 136 against 161, 24 of 1 to 700 90 against 101;
+    //   above: 16 of 1 to 2000, 52 tiles in the mean (group 6 of 64), 592 against 577; 128-wide, 37 tiles, 1044 against 893.
     const int64_t mean = tokens / std::max(sequences, 1);
-    const bool skewed = max_query > 0 && 4 * mean <= query && mean <= 8 * d->tile_tokens;
+    const bool skewed = max_query > 0 && 4 * mean <= query && mean <= (dim > 96 ? 3 : 8) * d->tile_tokens;
     const int tiles = query > d->tile_tokens && !skewed ? 2 : 1;
     d->unit_tokens = tiles * d->tile_tokens;
     d->tile_rows = 128;
