@@ -327,9 +327,10 @@ SVX_API int svx_paged_append(const svx_paged_cache* cache, const void* k, int64_
  * softmax(scale q k^T) v, kv head = q head / (q_heads / kv_heads). causal != 0: row i of a sequence with n new rows sees
  * the keys up to lengths - n + i; else all. A row that sees no key gives 0. lse (optional) [tokens][q_heads]: the natural
  * logarithm of the row's sum of exponentials, -inf for such a row. What the pages hold past a sequence's length is not
- * read. Lengths outside the table are clamped to it and page ids outside the pool count as keys and values of 0; both
- * set SVX_STATUS_BAD_PAGE. max_query: the most new rows of a sequence that the caller expects (0: unknown); it picks the
- * form of the kernel and never changes what is computed. workspace: svx_paged_attention_workspace_bytes of device
+ * read; a value that the causal mask hides from a row weighs 0 there (so a NaN among them is NaN in the row). Lengths outside
+ * the table are clamped to it and page ids outside the pool count as keys and values of 0; both set SVX_STATUS_BAD_PAGE.
+ * max_query: the most new rows of a sequence that the caller expects (0: unknown, the mean stands for it); it picks the form of
+ * the kernel, one for the whole call, and never changes what is computed. workspace: svx_paged_attention_workspace_bytes of device
  * scratch for the same arguments, for this call alone while it runs; nothing is kept in it between calls. */
 SVX_API size_t svx_paged_attention_workspace_bytes(int tokens, int sequences, int q_heads, int kv_heads, int dim,
                                                    int max_query);

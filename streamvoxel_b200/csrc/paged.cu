@@ -17,8 +17,8 @@
 // stages, so the loop has no block barrier; the warps' parts of a unit are merged through shared memory at its end.
 //
 // Measured on B200 (bf16 unless said): 128 sequences of 40 to 16,384 keys, 8 kv heads of 128, 4 query heads each, pages of
-// 16: 279 us, 5.6 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 213 us, 6.1 TB/s; one of 4001
-// keys, 8 heads of 128: 11.5 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
+// 16: 275 to 284 us, 5.6 TB/s; three of 90,000 to 131,072, 16 heads of 64 in fp16, pages of 128: 212 to 219 us, 6.1 TB/s; one
+// of 4001 keys, 8 heads of 128: 11.7 us, of which 1.5 are the plan, 1.8 the first page ids, 1.3 the keys, 1.2 the merge and 3.5 the
 // joining kernel with the gap before it.
 #include <math.h>
 

@@ -31,8 +31,9 @@
 // Bound: the tile loop, 1,540 (dim 128) to 1,740 (96) cycles for 256 rows x 64 keys, where products and softmax wait on one
 // another: the tensor pipe needs 1,280 or 960 of them (64-wide products of scores take 48 cycles for 32 of arithmetic), the
 // exponential unit 768. Without exponentials it ran 10% faster, without the maximum 2%. Measured on B200 (bf16): 4
-// chunks of 1500 to 2048 tokens x 32 heads of 128 over 9,000 to 32,768 keys, 8 kv heads, 1,190 to 1,260 us, 1,020 to 1,075
-// TFLOP/s under the power cap; 8 of 1024 rows x 8 heads of 96 over 2368 to 9536 keys without a mask 188 us, 700 TFLOP/s.
+// chunks of 1500 to 2048 tokens x 32 heads of 128 over 9,000 to 32,768 keys, 8 kv heads, 1,170 to 1,290 us, 990 to 1,095
+// TFLOP/s under the power cap; 8 of 1024 rows x 8 heads of 96 over 2368 to 9536 keys without a mask 182 to 190 us, 700 to
+// 730 TFLOP/s. The one-tile form spills 36 to 68 bytes a thread at the 128 registers that two CTAs a SM leave.
 //
 // Built, measured and not kept: two threads a row (16 softmax warps; 2,100 cycles a tile against 1,740: the warps of a
 // scheduler reach their exponentials together), and both chains on one query tile, every second key tile each (handing the

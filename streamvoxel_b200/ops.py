@@ -609,11 +609,13 @@ def paged_attention(q, k_pages, v_pages, table, lengths, offsets, *, causal=True
 
     q [tokens, q_heads, dim] (token and head strides multiples of 8), dim 64, 96 or 128, query head h reading kv head
     h // (q_heads / kv_heads). Sequence s's rows are its last tokens: causal, row i of n sees lengths[s] - n + i + 1 keys;
-    else all lengths[s]. A row that sees none gives 0. scale: 1 / sqrt(dim) unless given. Returns out [tokens, q_heads,
+    else all lengths[s]. A row that sees none gives 0; hidden keys weigh 0, so an infinite or NaN value among them is NaN in the
+    row. scale: 1 / sqrt(dim) unless given. Returns out [tokens, q_heads,
     dim] (contiguous, not overlapping q); rows outside of every sequence are left as they were. lse [tokens, q_heads]
     float32 (optional): the natural logarithm of the row's sum of exponentials, -inf for a row without keys.
     max_query: the most new tokens of a sequence in the batch, where the caller knows it; it picks the kernel's form, never
-    the result's meaning. workspace: from `paged_attention_workspace`, not shared by calls that may overlap; allocated
+    the result's meaning. Without it the mean decides, and a long chunk among single tokens may take the form for few rows
+    (2000 tokens and 199 single ones, 8 heads of 128: 382 us against 235). workspace: from `paged_attention_workspace`, not shared by calls that may overlap; allocated
     here unless given. status [sequences] int32 (optional) gets STATUS_BAD_PAGE where a page id lies outside the pool (read
     as zeros) or a length outside the table (clamped)."""
     cache = _paged_cache(k_pages, v_pages, table, lengths, offsets, status)
