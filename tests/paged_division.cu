@@ -1,5 +1,6 @@
 // The division of a batch of paged attention among CTAs, on the host: the arithmetic is that of the kernels (the host
 // side of paged.cuh); only the sums over the threads of a block are loops here.
+#include <algorithm>
 #include <vector>
 
 #include "paged.cuh"
@@ -7,7 +8,7 @@
 using namespace svx::paged;
 
 // shape: tokens, sequences, kv_heads, causal, unit_tokens, blocks, min_tiles, ctas, two_tiles (whole units are dealt out),
-// page_shift, table_width. segments: rows of 8 ints (cta, sequence, head, token tile, t0, t1, the unit's tiles, the partial
+// page_shift, table_width, threads (which add up equal numbers of sequences each). segments: rows of 8 ints (cta, sequence, head, token tile, t0, t1, the unit's tiles, the partial
 // that it leaves or -1); joins: rows of 5 (cta, parts, sequence, head, token tile) followed by `parts` partials. Returns
 // the segments' count, -1 when one of the arrays is too small; counts[0] = ints of joins, counts[1] = waves.
 extern "C" __attribute__((visibility("default"))) int paged_division(const int32_t* shape, const int32_t* lengths,
@@ -55,9 +56,14 @@ extern "C" __attribute__((visibility("default"))) int paged_division(const int32
     place.waves = waves;
     place.count = (int)(line[c + 1] - line[c]);
     if (place.count > 0) {
-      int s = 0;
-      while (before[s + 1] <= line[c]) ++s;
-      find_place(p, s, s + 1, load_sequence(p, s), before[s], line[c], each, c, waves ? line.data() : nullptr, &place);
+      const int per = (p.sequences + shape[11] - 1) / shape[11];
+      int s0 = 0;
+      while (before[std::min(p.sequences, s0 + per)] <= line[c]) s0 += per;
+      const int s1 = std::min(p.sequences, s0 + per);
+      int64_t tiles, units;
+      Sequence last;
+      add_sequences(p, s0, s1, &tiles, &units, &last);
+      find_place(p, s0, s1, last, before[s0], line[c], each, c, waves ? line.data() : nullptr, &place);
     }
     for (Walk w(p, place, c); w.more(); w.next(p, place, ctas)) {
       if (rows == segment_rows) return -1;

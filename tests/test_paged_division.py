@@ -24,12 +24,12 @@ def division(tmp_path_factory):
     assert result.returncode == 0, result.stderr
     call = ctypes.CDLL(target).paged_division
 
-    def run(news, lengths, kv_heads, unit_tokens, causal, *, ctas=SMS, two_tiles=True, min_tiles=4, blocks=1):
+    def run(news, lengths, kv_heads, unit_tokens, causal, *, ctas=SMS, two_tiles=True, min_tiles=4, blocks=1, threads=16):
         offsets = np.concatenate(([0], np.cumsum(news))).astype(np.int32)
         lengths = np.asarray(lengths, np.int32)
         width = max(1, -(-int(lengths.max()) // 16))
         shape = np.array([offsets[-1], len(news), kv_heads, causal, unit_tokens, blocks, min_tiles, ctas, two_tiles, 4,
-                          width], np.int32)
+                          width, threads], np.int32)
         units = sum(-(-int(n) // unit_tokens) for n in news) * kv_heads * blocks
         segments, joins = np.zeros((units + 2 * ctas, 8), np.int32), np.zeros(16 * ctas + 64, np.int32)
         counts = np.zeros(2, np.int32)
